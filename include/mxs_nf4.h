@@ -38,6 +38,7 @@ extern "C" {
 
 #define MXS_DTYPE_F16 0
 #define MXS_DTYPE_F32 1
+#define MXS_DTYPE_BF16 2 /* the optimizer's and the head's operands */
 
 /* Dense W from packed NF4.  Replaces unpack_nf4 (solution/nf4.py:138-155) with its
  * wide/one-byte dispatch (solution/nf4.py:145-154): the wide kernel when n_bytes % 32 == 0 and
@@ -600,6 +601,43 @@ int mxs_nf4_linear_glu_fused(int M, int N, int K, int bwd);
 
 /* dst[cols, rows] = src[rows, cols]^T, fp16 (lora_A -> the [K, r] operand of the backward). */
 int mxs_transpose_f16(const void* src, int rows, int cols, void* dst, hipStream_t stream);
+
+/* ---- the end of a training step -------------------------------------------------------------
+ *
+ * Tensors of several calls are lists: `count` pointers (device) and value counts (host arrays).
+ * dtypes[i]: MXS_DTYPE_F16 / F32 / BF16 of tensor i.  Lists of any length; a size may be 0. */
+
+/* out[0] (fp32, device) = the 2-norm over all values of `grads`, divided by grad_scale[0] (device)
+ * if that is not NULL.  Squares and sums in fp64, in a fixed order.  workspace:
+ * mxs_grad_norm_workspace_bytes(count, sizes), 8-byte aligned. */
+int64_t mxs_grad_norm_workspace_bytes(int count, const int64_t* sizes);
+int mxs_grad_norm(int count, const void* const* grads, const int64_t* sizes, const int* dtypes,
+                  const float* grad_scale, float* out, void* workspace, hipStream_t stream);
+
+/* One AdamW step (decoupled weight decay) over `count` parameter tensors, in place.  step[0]
+ * (fp32, device) is the number of steps so far; it becomes t = step[0] + 1.  With
+ * c = min(1, max_norm / (norm[0] + 1e-6)) / grad_scale[0] (norm, grad_scale: device, each 1 where
+ * NULL), g = grad * c:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps).
+ * lr_dev (device) overrides lr.  found_inf[0] != 0 (device) leaves everything as it was.
+ * grads[i] has params[i]'s dtype.  state_bits 32: m, v fp32.  state_bits 8: m, v u8 codes and one
+ * fp32 scale per 256 values (avg_scales[i], avg_sq_scales[i], ceil(size / 256) each): value =
+ * scale * book[code], m over the signed and v over the unsigned 8-bit dynamic map; the new scale
+ * is the block's largest magnitude (NaN when a value is not finite) and the new code the nearest
+ * one, the lower of two as near, decided in fp64.  No two written tensors may overlap.
+ * workspace: 64 bytes, 8-byte aligned. */
+int mxs_adamw_step(int count, void* const* params, const void* const* grads, void* const* avgs,
+                   void* const* avg_sqs, float* const* avg_scales, float* const* avg_sq_scales,
+                   const int64_t* sizes, const int* dtypes, int state_bits, float* step, double lr,
+                   const float* lr_dev, double beta1, double beta2, double eps,
+                   double weight_decay, const float* norm, double max_norm,
+                   const float* grad_scale, const float* found_inf, void* workspace,
+                   hipStream_t stream);
+
+/* out[n] (fp32) = the values of n 8-bit state codes: book[codes[i]] * scale[i / 256]. */
+int mxs_state_values(const void* codes, const float* scale, int64_t n, int is_signed, float* out,
+                     hipStream_t stream);
 
 #ifdef __cplusplus
 }

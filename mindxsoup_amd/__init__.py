@@ -27,6 +27,7 @@ FEATURES = {
     "stream_weights": False,  # decoder NF4 weights in pinned host memory, a layer at a time
     "torch_ops": True,       # projections on the compiled torch.ops.mxs_nf4 operators (C++
                              # host side and autograd); False: Python Functions over ctypes
+    "fused_adamw": False,    # transformers' Trainer on optim.AdamW (fp32 or 8-bit states)
     # --- reference switches outside the NF4 path (inert here) ------------------------------
     "startup_cache": False, "example_swiglu": False, "adam_host": False,
     "cublas_workspace": None, "fused_layer_input": False, "fused_head_acc": False,
@@ -79,3 +80,7 @@ def apply():
         from . import attention
 
         attention.patch_qwen2_attention_fp16()
+    if FEATURES["fused_adamw"]:
+        from . import optim
+
+        optim.patch_trainer()

@@ -16,6 +16,7 @@ LIB_PATH = os.environ.get("MXS_NF4_LIB") or \
 
 MXS_DTYPE_F16 = 0
 MXS_DTYPE_F32 = 1
+MXS_DTYPE_BF16 = 2
 
 _ERRORS = {-1: "bad argument (null pointer or negative size)", -2: "unsupported dtype",
            -3: "pointer alignment", -4: "shape outside what the kernels take"}
@@ -31,6 +32,7 @@ P = ctypes.c_void_p
 I64 = ctypes.c_int64
 I32 = ctypes.c_int
 F32 = ctypes.c_float
+F64 = ctypes.c_double
 
 # name -> argtypes (all return int)
 _SIGNATURES = {
@@ -107,6 +109,11 @@ _SIGNATURES = {
     "mxs_nf4_linear_route": [I32, I32, I32, I32, I32],
     "mxs_nf4_linear_bwd_dx_pair_ok": [I32, I32, I32, I32],
     "mxs_nf4_linear_bwd_dx_pair_workspace_bytes": [I32, I32, I32, I32],
+    "mxs_grad_norm_workspace_bytes": [I32, P],
+    "mxs_grad_norm": [I32, P, P, P, P, P, P, P],
+    "mxs_adamw_step": [I32, P, P, P, P, P, P, P, P, I32, P, F64, P, F64, F64, F64, F64, P, F64, P,
+                       P, P, P],
+    "mxs_state_values": [P, P, I64, I32, P, P],
 }
 
 
@@ -115,7 +122,8 @@ _RESTYPES = {"mxs_nf4_dequant_layer_plan": ctypes.c_int64,
              "mxs_lora_workspace_bytes": ctypes.c_int64,
              "mxs_nf4_linear_fwd_group_workspace_bytes": ctypes.c_int64,
              "mxs_nf4_linear_bwd_dx_sum_workspace_bytes": ctypes.c_int64,
-             "mxs_nf4_linear_bwd_dx_pair_workspace_bytes": ctypes.c_int64}
+             "mxs_nf4_linear_bwd_dx_pair_workspace_bytes": ctypes.c_int64,
+             "mxs_grad_norm_workspace_bytes": ctypes.c_int64}
 
 
 def lib():

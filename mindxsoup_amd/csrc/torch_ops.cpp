@@ -17,6 +17,7 @@
 //   lora_fwd_group    lora_fwd for 1..4 projections reading one input (q/k/v; gate/up)
 //   lora_bwd_group    lora_bwd for them, small launches shared
 //   mlp_fwd, mlp_bwd  the SwiGLU MLP block of three such projections (solution/mlp.py:33-44)
+//   grad_norm, adamw_step, state_values  the end of a training step over lists of tensors
 // Autograd ops (one node per call; backward in C++), named as the package's Python Functions
 // they stand for (a node's name() says which ran):
 //   linear         NF4LinearFunction
@@ -33,6 +34,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <array>
 #include <optional>
 #include <tuple>
@@ -1521,6 +1523,188 @@ std::vector<Tensor> lora_siblings_plain(const Tensor& x, TensorList lora_a, Tens
                               keep, mask_scale, s, one_gemm, cos, sin, n_rope));
 }
 
+// ---- the end of a training step ---------------------------------------------------------------
+
+int float_dtype(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kHalf: return MXS_DTYPE_F16;
+    case at::kFloat: return MXS_DTYPE_F32;
+    case at::kBFloat16: return MXS_DTYPE_BF16;
+    default: TORCH_CHECK(false, name, " must be fp32, fp16 or bf16, got ", t.scalar_type());
+  }
+}
+
+// An optional fp32 scalar in device memory.
+const float* scalar_ptr(const OptTensor& t, const at::Device& dev, const char* name) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  TORCH_CHECK(t->scalar_type() == at::kFloat && t->numel() == 1 && t->device() == dev, name,
+              " must be one fp32 value on ", dev, ", got ", t->scalar_type(), " ", t->sizes(),
+              " on ", t->device());
+  return t->data_ptr<float>();
+}
+
+
+
+Tensor grad_norm_cuda(TensorList grads, const OptTensor& grad_scale) {
+  TORCH_CHECK(!grads.empty(), "grads must hold at least one tensor");
+  const at::Device dev = grads[0].device();
+  const at::OptionalDeviceGuard guard(dev);
+  const size_t n = grads.size();
+  std::vector<Tensor> kept;  // copies of the tensors that are not dense
+  std::vector<const void*> g(n);
+  std::vector<int64_t> sizes(n);
+  std::vector<int> dtypes(n);
+  for (size_t i = 0; i < n; i++) {
+    TORCH_CHECK(grads[i].device() == dev, "grads[", i, "] must be on ", dev, ", found ",
+                grads[i].device());
+    dtypes[i] = float_dtype(grads[i], "grads");
+    const bool direct = grads[i].is_non_overlapping_and_dense();
+    if (!direct) kept.push_back(grads[i].contiguous());
+    g[i] = (direct ? grads[i] : kept.back()).data_ptr();
+    sizes[i] = grads[i].numel();
+  }
+  const int count = as_int((int64_t)n, "the number of gradients");
+  const float* scale = scalar_ptr(grad_scale, dev, "grad_scale");
+  Tensor out = at::empty({}, grads[0].options().dtype(at::kFloat));
+  Tensor ws = at::empty({mxs_grad_norm_workspace_bytes(count, sizes.data())},
+                        out.options().dtype(at::kByte));
+  ok(mxs_grad_norm(count, g.data(), sizes.data(), dtypes.data(), scale, out.data_ptr<float>(),
+                   ws.data_ptr(), stream_of(out)),
+     "mxs_grad_norm");
+  return out;
+}
+
+Tensor grad_norm_meta(TensorList grads, const OptTensor&) {
+  TORCH_CHECK(!grads.empty(), "grads must hold at least one tensor");
+  return at::empty({}, grads[0].options().dtype(at::kFloat));
+}
+
+constexpr int64_t kStateBlock = 256;  // 8-bit values per scale
+
+void adamw_step_cuda(TensorList params, TensorList grads, TensorList avgs, TensorList avg_sqs,
+                     TensorList avg_scales, TensorList avg_sq_scales, const Tensor& step,
+                     double lr, const OptTensor& lr_dev, double beta1, double beta2, double eps,
+                     double weight_decay, const OptTensor& norm, double max_norm,
+                     const OptTensor& grad_scale, const OptTensor& found_inf) {
+  const size_t n = params.size();
+  TORCH_CHECK(grads.size() == n && avgs.size() == n && avg_sqs.size() == n,
+              "params, grads, exp_avgs and exp_avg_sqs must be as many: ", n, ", ", grads.size(),
+              ", ", avgs.size(), ", ", avg_sqs.size());
+  const at::Device dev = step.device();
+  const at::OptionalDeviceGuard guard(dev);
+  TORCH_CHECK(step.scalar_type() == at::kFloat && step.numel() == 1,
+              "step must be one fp32 value, got ", step.scalar_type(), " ", step.sizes());
+  const bool bits8 = n && avgs[0].scalar_type() == at::kByte;
+  const size_t scales = bits8 ? n : 0;
+  TORCH_CHECK(avg_scales.size() == scales && avg_sq_scales.size() == scales,
+              bits8 ? "8-bit states need one tensor of scales each: "
+                    : "32-bit states take no scales: ",
+              avg_scales.size(), ", ", avg_sq_scales.size());
+  std::vector<Tensor> kept;  // gradients laid out like their parameters
+  std::vector<void*> p(n), m(n), v(n);
+  std::vector<const void*> g(n);
+  std::vector<float*> ms(scales), vs(scales);
+  std::vector<int64_t> sizes(n);
+  std::vector<int> dtypes(n);
+  using Range = std::pair<uintptr_t, uintptr_t>;
+  std::vector<Range> written;
+  written.reserve(5 * n + 1);
+  auto writes = [&](const Tensor& t) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
+    if (t.numel()) written.push_back({at, at + t.nbytes()});
+  };
+  const auto state = bits8 ? at::kByte : at::kFloat;
+  for (size_t i = 0; i < n; i++) {
+    const Tensor &pi = params[i], &gi = grads[i], &mi = avgs[i], &vi = avg_sqs[i];
+    TORCH_CHECK(pi.is_non_overlapping_and_dense(), "params[", i,
+                "] must lie in one piece of memory, got strides ", pi.strides());
+    for (const Tensor* t : {&pi, &gi, &mi, &vi}) {
+      TORCH_CHECK(t->device() == dev, "tensors ", i, " must be on ", dev, ", found ",
+                  t->device());
+      TORCH_CHECK(t->sizes() == pi.sizes(), "tensors ", i, " must be ", pi.sizes(), ", got ",
+                  t->sizes());
+    }
+    dtypes[i] = float_dtype(pi, "params");
+    TORCH_CHECK(gi.scalar_type() == pi.scalar_type(), "grads[", i, "] must be ",
+                pi.scalar_type(), ", got ", gi.scalar_type());
+    for (const Tensor* t : {&mi, &vi}) {
+      TORCH_CHECK(t->scalar_type() == state, "states ", i, " must be ", state,
+                  " like the first one, got ", t->scalar_type());
+      TORCH_CHECK(t->strides() == pi.strides(), "states ", i, " must have strides ",
+                  pi.strides(), ", got ", t->strides());
+    }
+    if (bits8) {
+      const int64_t blocks = (pi.numel() + kStateBlock - 1) / kStateBlock;
+      for (const Tensor* t : {&avg_scales[i], &avg_sq_scales[i]})
+        TORCH_CHECK(t->device() == dev && t->scalar_type() == at::kFloat &&
+                        t->is_contiguous() && t->dim() == 1 && t->numel() == blocks,
+                    "scales ", i, " must be fp32 [", blocks, "] on ", dev, ", got ",
+                    t->scalar_type(), " ", t->sizes());
+      ms[i] = avg_scales[i].data_ptr<float>();
+      vs[i] = avg_sq_scales[i].data_ptr<float>();
+      writes(avg_scales[i]);
+      writes(avg_sq_scales[i]);
+    }
+    const bool direct = gi.strides() == pi.strides();
+    if (!direct) {
+      kept.push_back(at::empty_strided(pi.sizes(), pi.strides(), pi.options()));
+      kept.back().copy_(gi);
+    }
+    p[i] = pi.data_ptr();
+    g[i] = (direct ? gi : kept.back()).data_ptr();
+    m[i] = mi.data_ptr();
+    v[i] = vi.data_ptr();
+    sizes[i] = pi.numel();
+    for (const Tensor* t : {&pi, &mi, &vi}) writes(*t);
+  }
+  writes(step);
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); i++)
+    TORCH_CHECK(written[i - 1].second <= written[i].first,
+                "two of the tensors that the step writes overlap");
+  const int count = as_int((int64_t)n, "the number of parameters");
+  Tensor ws = at::empty({64}, step.options().dtype(at::kByte));
+  ok(mxs_adamw_step(count, p.data(), g.data(), m.data(), v.data(), ms.data(), vs.data(),
+                    sizes.data(), dtypes.data(), bits8 ? 8 : 32, step.data_ptr<float>(), lr,
+                    scalar_ptr(lr_dev, dev, "lr"), beta1, beta2, eps, weight_decay,
+                    scalar_ptr(norm, dev, "norm"), max_norm,
+                    scalar_ptr(grad_scale, dev, "grad_scale"),
+                    scalar_ptr(found_inf, dev, "found_inf"), ws.data_ptr(), stream_of(step)),
+     "mxs_adamw_step");
+  // the written tensors have a new version: a graph that saved one of them notices
+  for (TensorList list : {params, avgs, avg_sqs, avg_scales, avg_sq_scales})
+    for (const Tensor& t : list)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  if (!step.is_inference()) step.unsafeGetTensorImpl()->bump_version();
+}
+
+void adamw_step_meta(TensorList, TensorList, TensorList, TensorList, TensorList, TensorList,
+                     const Tensor&, double, const OptTensor&, double, double, double, double,
+                     const OptTensor&, double, const OptTensor&, const OptTensor&) {}
+
+Tensor state_values_meta(const Tensor& codes, const Tensor& scale, bool) {
+  TORCH_CHECK(codes.scalar_type() == at::kByte, "codes must be uint8, got ",
+              codes.scalar_type());
+  const int64_t blocks = (codes.numel() + kStateBlock - 1) / kStateBlock;
+  TORCH_CHECK(scale.scalar_type() == at::kFloat && scale.dim() == 1 && scale.numel() == blocks &&
+                  scale.device() == codes.device(),
+              "scale must be fp32 [", blocks, "] on ", codes.device(), ", got ",
+              scale.scalar_type(), " ", scale.sizes(), " on ", scale.device());
+  TORCH_CHECK(codes.is_non_overlapping_and_dense(),
+              "codes must lie in one piece of memory, got strides ", codes.strides());
+  return at::empty_strided(codes.sizes(), codes.strides(), codes.options().dtype(at::kFloat));
+}
+
+Tensor state_values_cuda(const Tensor& codes, const Tensor& scale, bool is_signed) {
+  const at::OptionalDeviceGuard guard(codes.device());
+  const Tensor s = scale.contiguous();
+  Tensor out = state_values_meta(codes, s, is_signed);
+  ok(mxs_state_values(codes.data_ptr(), s.data_ptr<float>(), codes.numel(), is_signed ? 1 : 0,
+                      out.data_ptr<float>(), stream_of(codes)),
+     "mxs_state_values");
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(mxs_nf4, m) {
@@ -1561,6 +1745,13 @@ TORCH_LIBRARY(mxs_nf4, m) {
         "Tensor[] absmax8, Tensor[] code, Tensor[] absmax2, Tensor[] offset, Tensor?[] bias, "
         "Tensor?[] keep, float mask_scale, float s, bool one_gemm, Tensor? cos=None, "
         "Tensor? sin=None, int n_rope=0) -> Tensor[]");
+  m.def("grad_norm(Tensor[] grads, Tensor? grad_scale) -> Tensor");
+  m.def("adamw_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avgs, "
+        "Tensor(c!)[] exp_avg_sqs, Tensor(d!)[] avg_scales, Tensor(e!)[] avg_sq_scales, "
+        "Tensor(f!) step, float lr, Tensor? lr_dev, float beta1, float beta2, float eps, "
+        "float weight_decay, Tensor? norm, float max_norm, Tensor? grad_scale, "
+        "Tensor? found_inf) -> ()");
+  m.def("state_values(Tensor codes, Tensor scale, bool signed) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(mxs_nf4, CUDA, m) {
@@ -1573,6 +1764,9 @@ TORCH_LIBRARY_IMPL(mxs_nf4, CUDA, m) {
   m.impl("lora_bwd_group", &lora_bwd_group_cuda);
   m.impl("mlp_fwd", &mlp_fwd_cuda);
   m.impl("mlp_bwd", &mlp_bwd_cuda);
+  m.impl("grad_norm", &grad_norm_cuda);
+  m.impl("adamw_step", &adamw_step_cuda);
+  m.impl("state_values", &state_values_cuda);
 }
 
 TORCH_LIBRARY_IMPL(mxs_nf4, Meta, m) {
@@ -1585,6 +1779,9 @@ TORCH_LIBRARY_IMPL(mxs_nf4, Meta, m) {
   m.impl("lora_bwd_group", &lora_bwd_group_meta);
   m.impl("mlp_fwd", &mlp_fwd_meta);
   m.impl("mlp_bwd", &mlp_bwd_meta);
+  m.impl("grad_norm", &grad_norm_meta);
+  m.impl("adamw_step", &adamw_step_meta);
+  m.impl("state_values", &state_values_meta);
 }
 
 // The autograd ops: the same node with or without grad mode (without it, or with no input
