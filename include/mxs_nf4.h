@@ -639,6 +639,30 @@ int mxs_adamw_step(int count, void* const* params, const void* const* grads, voi
 int mxs_state_values(const void* codes, const float* scale, int64_t n, int is_signed, float* out,
                      hipStream_t stream);
 
+/* The language-model head with its softmax cross entropy (solution/fused_ce.py:95-148, FusedHeadCE),
+ * without the matrix of logits: for h [T, D] (row stride ldh), w [V, D] (row stride ldw) and
+ * int64 labels [T], loss_t = log(sum_v exp(h_t . w_v)) - h_t . w_y, 0 for rows whose label is
+ * ignore_index, NaN (with NaN gradients) for labels outside [0, V).
+ *   dtype      MXS_DTYPE_F16 or MXS_DTYPE_BF16 of h and w
+ *   reduction  0: loss fp32 [T];  1: loss fp32 [1], the sum;  2: their mean over the rows that
+ *              have a label (NaN if none has)
+ *   dh, dw     fp32 [T, D] and [V, D], each may be NULL: the gradients of the sum (0, 1) or the mean
+ *              (2) of the losses; with row_grad (fp32 [T], may be NULL) row t's part times
+ *              row_grad[t].  dw under reduction 0 needs row_grad.  loss may be NULL then.
+ * D % 64 == 0; w 16-byte aligned with ldw % 8 == 0; dh, dw 16-byte aligned.  workspace:
+ * mxs_head_ce_workspace_bytes(...), 256-byte aligned; at most about 1 GiB of 16-bit exponentials
+ * (more rows are worked through in pieces), unless 256 rows of them are more. */
+int64_t mxs_head_ce_workspace_bytes(int T, int V, int D, int want_dh, int want_dw);
+int mxs_head_ce(const void* h, int64_t ldh, const void* w, int64_t ldw, const int64_t* labels,
+                int T, int V, int D, int dtype, int64_t ignore_index, int reduction,
+                const float* row_grad, float* loss, float* dh, float* dw, void* workspace,
+                hipStream_t stream);
+
+/* out [rows, cols] (fp16 or bf16) = unit (fp32) * g[0], or g[row] with per_row: the gradient that
+ * mxs_head_ce left, times the one that came from above.  cols % 8 == 0, 16-byte aligned. */
+int mxs_head_ce_grad(const float* unit, const float* g, int per_row, int64_t rows, int cols,
+                     int dtype, void* out, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

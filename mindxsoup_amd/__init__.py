@@ -27,13 +27,14 @@ FEATURES = {
     "stream_weights": False,  # decoder NF4 weights in pinned host memory, a layer at a time
     "torch_ops": True,       # projections on the compiled torch.ops.mxs_nf4 operators (C++
                              # host side and autograd); False: Python Functions over ctypes
+    "fused_ce": False,       # Qwen2's training loss from the head without its logits (fused_ce.py)
     "fused_adamw": False,    # transformers' Trainer on optim.AdamW (fp32 or 8-bit states)
     # --- reference switches outside the NF4 path (inert here) ------------------------------
     "startup_cache": False, "example_swiglu": False, "adam_host": False,
     "cublas_workspace": None, "fused_layer_input": False, "fused_head_acc": False,
     "lean_draw": False, "mlp_gateup_recompute": False, "mlp_tail": False, "rmsnorm": False,
     "rope": False,  # the RoPE-only patch of apply_rotary_pos_emb; attention_fp16 rotates instead
-    "fused_ce": False, "fp16_embedding": False, "head_stream": False,
+    "fp16_embedding": False, "head_stream": False,
     "head_slice": 4096, "unpad": False, "recompute": False,
     "recompute_fp16_inputs": False, "recompute_host_inputs": False,
     "recompute_group_tokens": 0, "recompute_no_rerun": False, "offload_activations": False,
@@ -80,6 +81,10 @@ def apply():
         from . import attention
 
         attention.patch_qwen2_attention_fp16()
+    if FEATURES["fused_ce"]:
+        from . import fused_ce
+
+        fused_ce.patch_qwen2_head_ce()
     if FEATURES["fused_adamw"]:
         from . import optim
 

@@ -114,6 +114,9 @@ _SIGNATURES = {
     "mxs_adamw_step": [I32, P, P, P, P, P, P, P, P, I32, P, F64, P, F64, F64, F64, F64, P, F64, P,
                        P, P, P],
     "mxs_state_values": [P, P, I64, I32, P, P],
+    "mxs_head_ce_workspace_bytes": [I32, I32, I32, I32, I32],
+    "mxs_head_ce": [P, I64, P, I64, P, I32, I32, I32, I32, I64, I32, P, P, P, P, P, P],
+    "mxs_head_ce_grad": [P, P, I32, I64, I32, I32, P, P],
 }
 
 
@@ -123,7 +126,8 @@ _RESTYPES = {"mxs_nf4_dequant_layer_plan": ctypes.c_int64,
              "mxs_nf4_linear_fwd_group_workspace_bytes": ctypes.c_int64,
              "mxs_nf4_linear_bwd_dx_sum_workspace_bytes": ctypes.c_int64,
              "mxs_nf4_linear_bwd_dx_pair_workspace_bytes": ctypes.c_int64,
-             "mxs_grad_norm_workspace_bytes": ctypes.c_int64}
+             "mxs_grad_norm_workspace_bytes": ctypes.c_int64,
+             "mxs_head_ce_workspace_bytes": ctypes.c_int64}
 
 
 def lib():

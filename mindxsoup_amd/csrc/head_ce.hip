@@ -1,0 +1,1152 @@
+// The language-model head with its softmax cross entropy on gfx950: for hidden states h [T, D], a
+// table W [V, D] and labels y, the losses l_t = log(sum_v exp(z_tv)) - z_ty of z = h W^T, and the
+// gradients dh = dz W and dW = dz^T h of dz = softmax(z) - onehot(y).  The logits never exist as
+// a matrix: a product's tile leaves its largest value and its sum of exponentials per row, and,
+// where gradients are wanted, its exponentials in 16 bits, for at most kPieceBytes of them at a
+// time (a piece of the rows); the gradients are products over those.
+//
+// Rows whose label is to be ignored are taken out first (k_ce_rows gathers the others), so they cost
+// nothing and what they hold (infinities, NaN) reaches nothing.
+//
+// Bound by MFMA: 2 T V D operations per product (one for the losses, a second and third for dh and
+// dW), at few rows by reading the table once.  All three products run on one engine
+// (stream_tiles): persistent workgroups of eight waves, direct global -> LDS copies of both
+// operands that run ahead over tile borders, so that only the first tile of a workgroup waits for
+// its operands, and an epilogue from registers while the next tile's copies land.
+#include "common.h"
+#include "mxs_nf4.h"
+
+namespace mxs {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kK = 64;             // reduction step: four MFMAs of 16
+constexpr int kWaves = 8;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kRowPad = 256;       // gathered rows are padded with zeros to a multiple of this
+constexpr int kVocabTile = 256;    // vocabulary columns of a logits tile
+constexpr int64_t kPieceBytes = (int64_t)1 << 30;  // 16-bit exponentials held at a time
+
+// ---- element types ----------------------------------------------------------------------------
+
+template <typename T>
+struct Elem;
+// Exponentials relative to a power of two are in (0, 1]: times 2^15 they use fp16's whole range
+// (normal down to 2^-29); dz in [-1, 1] is kept times 2^14.
+template <>
+struct Elem<_Float16> {
+  static constexpr float kExpBits = 15.0f, kGradBits = 14.0f;
+  static __device__ __forceinline__ float16_t mma(u32x4 a, u32x4 b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a),
+                                                  __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    return pack_f16x2(lo, hi);
+  }
+};
+template <>
+struct Elem<__bf16> {
+  static constexpr float kExpBits = 0.0f, kGradBits = 0.0f;
+  static __device__ __forceinline__ float16_t mma(u32x4 a, u32x4 b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    bf16x2 v = {(__bf16)lo, (__bf16)hi};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+};
+
+// ---- what the kernels of a call share -----------------------------------------------------------
+
+struct RowStat {
+  float top;    // whole power of two that the row's sum is relative to
+  float inv;    // 1 / sum of 2^(z log2 e - top)
+  float miss;   // 1 - p of the label
+  float loss;
+};
+
+struct CeArgs {
+  const void* h;
+  int64_t ldh;
+  const void* w;
+  int64_t ldw;
+  const int64_t* labels;
+  int64_t ignore;
+  int T, V, D;
+  const float* row_grad;
+  float* loss;   // [T] or [1]
+  float* dh;     // [T, D] or null
+  float* dw;     // [V, D] or null
+  int mean, per_row;
+  // workspace
+  int* count;        // rows with a label
+  float* gmax;       // largest |row_grad| of them
+  int* idx;          // [Tp] their rows in h
+  int* lab;          // [Tp] their labels; -1 behind the last, -2 outside the vocabulary
+  void* hc;          // [Tp, D] gathered
+  RowStat* row;      // [Tp]
+  float* zy;         // [Tp] the label's logit
+  float2* stat;      // [blocks][piece rows] power of two and sum of a block of columns
+  u32x4* e;          // [Vp / 64][piece rows / 32][4][64] fragments of exponentials, then dz
+  float* part;       // [splits][piece rows][D]
+  // the piece
+  int row0, rows;    // first gathered row, rows (a multiple of kRowPad)
+  int first;         // the call's first piece
+  int stat_cols;     // columns of a block of `stat`
+  int splits, split_steps;
+};
+
+__device__ __forceinline__ int piece_rows(const CeArgs& a) {
+  return min(max(a.count[0] - a.row0, 0), a.rows);
+}
+
+// ---- rows with a label ------------------------------------------------------------------------
+
+constexpr int kGather = 32;  // gathered rows of a workgroup
+
+// Gathers the rows whose label is not `ignore`, in order, and pads with zeros.  Every workgroup
+// counts all the labels itself (an L2 read of 8 T bytes; one launch, no waiting on another
+// workgroup) and copies its own rows.  Ignored rows get their zeros in loss and dh here.
+__global__ __launch_bounds__(256) void k_ce_rows(CeArgs a, int vec) {
+  __shared__ int s_sum[256], s_idx[kGather];
+  const int t = threadIdx.x, r0 = (int)blockIdx.x * kGather;
+  const int per = (a.T + 255) / 256, t0 = min(t * per, a.T), t1 = min(t0 + per, a.T);
+  int n = 0;
+  for (int i = t0; i < t1; i++) n += a.labels[i] != a.ignore ? 1 : 0;
+  s_sum[t] = n;
+  if (t < kGather) s_idx[t] = -1;
+  __syncthreads();
+  for (int o = 1; o < 256; o <<= 1) {
+    const int v = t >= o ? s_sum[t - o] : 0;
+    __syncthreads();
+    s_sum[t] += v;
+    __syncthreads();
+  }
+  if (r0 == 0 && t == 0) a.count[0] = s_sum[255];
+  int at = s_sum[t] - n;
+  if (at < r0 + kGather && at + n > r0)
+    for (int i = t0; i < t1; i++)
+      if (a.labels[i] != a.ignore) {
+        if (at >= r0 && at < r0 + kGather) s_idx[at - r0] = i;
+        at++;
+      }
+  __syncthreads();
+  if (t < kGather) {
+    const int i = s_idx[t];
+    int y = -1;
+    if (i >= 0) {
+      const int64_t l = a.labels[i];
+      y = l >= 0 && l < a.V ? (int)l : -2;
+    }
+    a.idx[r0 + t] = i;
+    a.lab[r0 + t] = y;
+  }
+  const int chunks = a.D / 8;  // 16-byte pieces of a row
+  u32x4* out = static_cast<u32x4*>(a.hc) + (int64_t)r0 * chunks;
+  for (int c = t; c < kGather * chunks; c += 256) {
+    const int r = c / chunks, k = c - r * chunks, i = s_idx[r];
+    u32x4 v = {0, 0, 0, 0};
+    if (i >= 0) {
+      const uint16_t* src = static_cast<const uint16_t*>(a.h) + (int64_t)i * a.ldh + 8 * k;
+      if (vec) {
+        v = *reinterpret_cast<const u32x4*>(src);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; q++) v[q] = src[2 * q] | ((uint32_t)src[2 * q + 1] << 16);
+      }
+    }
+    out[c] = v;
+  }
+  for (int r = 0; r < kGather; r++) {
+    const int i = r0 + r;
+    if (i >= a.T || a.labels[i] != a.ignore) continue;
+    if (a.per_row && a.loss && t == 0) a.loss[i] = 0.0f;
+    if (a.dh)
+      for (int k = t; k < a.D / 4; k += 256)
+        reinterpret_cast<float4_t*>(a.dh + (int64_t)i * a.D)[k] = (float4_t){0, 0, 0, 0};
+  }
+}
+
+// Largest |row_grad| of the rows with a label: dz is kept relative to it, in fp16's range.
+__global__ __launch_bounds__(1024) void k_ce_gmax(CeArgs a) {
+  __shared__ float s[1024];
+  const int t = threadIdx.x;
+  float m = 0.0f;
+  for (int i = t; i < a.T; i += 1024)
+    if (a.labels[i] != a.ignore) {
+      const float g = fabsf(a.row_grad[i]);
+      m = (m > g || m != m) ? m : g;
+    }
+  s[t] = m;
+  __syncthreads();
+  for (int o = 512; o; o >>= 1) {
+    if (t < o) {
+      const float g = s[t + o];
+      m = (m > g || m != m) ? m : g;
+      s[t] = m;
+    }
+    __syncthreads();
+  }
+  if (t == 0) a.gmax[0] = m;
+}
+
+// ---- the engine -------------------------------------------------------------------------------
+
+// One 1 KB direct copy: 16 bytes per lane from base + off to consecutive LDS addresses.  Inline
+// asm, so that the compiler's own waits do not count it; completion is awaited by hand.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void copy1k(uint32_t lds, const void* base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+  return __builtin_amdgcn_readfirstlane(
+      static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)));
+}
+
+__device__ __forceinline__ u32x2 read_tr(const char* p) {
+  typedef __attribute__((address_space(3))) short4_t lds_short4;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)p));
+}
+
+// An operand [ROWS][kK] whose reduction index is contiguous.  128-byte LDS rows of eight 16-byte
+// segments, segment s of row r at s ^ (r / 2 % 8): the 32 rows of a fragment read then fall on
+// all banks alike.  A fragment: row lane % 32, reduction indexes 8 (lane / 32) .. + 7.
+template <int ROWS>
+struct RowTile {
+  static constexpr int BYTES = ROWS * kK * 2, N = (ROWS + 63) / 64;
+  uint32_t off[N];
+  const char* base;
+  int read0;  // byte offset of the lane's row and (first) segment
+
+  // rows row0 .. of src, those past `last` repeating it
+  __device__ __forceinline__ void tile(const void* src, int64_t ld, int row0, int last, int wave,
+                                       int lane) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int row = (wave * 8 + 64 * i + (lane >> 3)) % ROWS;
+      const int seg = ((lane & 7) ^ (row >> 1)) & 7;
+      off[i] = ((uint32_t)min(row, last - row0) * (uint32_t)ld + seg * 8) * 2;
+    }
+    base = static_cast<const char*>(src) + (int64_t)row0 * ld * 2;
+  }
+  __device__ __forceinline__ void copy(uint32_t lds, int k, int i, int wave) const {
+    copy1k(lds + (wave * 8 + 64 * i) % ROWS * 128, base + (int64_t)k * (kK * 2), off[i]);
+  }
+  __device__ __forceinline__ static u32x4 read(const char* s, int row0, int kk, int lane) {
+    const int row = row0 + (lane & 31);
+    const int seg = (2 * kk + (lane >> 5)) ^ ((row >> 1) & 7);
+    return *reinterpret_cast<const u32x4*>(s + row * 128 + seg * 16);
+  }
+};
+
+// An operand [kK][COLS] whose reduction index is the row, read through the transposing LDS read.
+// LDS rows of COLS / 8 segments, rotated by four for every row of a group of four (two where the
+// row length already puts odd rows on the other half of the banks).  A fragment: column
+// lane % 32, reduction indexes 4 h .. + 3 and 8 + 4 h .. + 3 of its 16 (h = lane / 32).
+template <int COLS>
+struct ColTile {
+  static constexpr int BYTES = COLS * kK * 2, N = COLS / 64, SEGS = COLS / 8;
+  static constexpr bool kHalf = COLS % 128 != 0;  // 64-column multiples: rows 32 dwords apart
+  int row_[N], seg8[N];
+  const char* base;
+  int64_t ld2;
+
+  __device__ __forceinline__ static int rot(int row) {
+    return kHalf ? ((row >> 1) & 1) * 4 : (row & 3) * 4;
+  }
+  // columns col0 .. of src (whole segments; those past the end repeat the last one)
+  __device__ __forceinline__ void tile(const void* src, int64_t ld, int col0, int cols, int wave,
+                                       int lane) {
+    ld2 = ld * 2;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int q = (wave + kWaves * i) * 64 + lane;
+      const int row = q / SEGS, p = q % SEGS;
+      const int seg = (p + SEGS - rot(row) % SEGS) % SEGS;
+      row_[i] = row;
+      seg8[i] = min(seg * 8, cols - 8 - col0) * 2;
+    }
+    base = static_cast<const char*>(src) + (int64_t)col0 * 2;
+  }
+  // rows kK k .. of the operand, those past `last` repeating it
+  __device__ __forceinline__ void copy(uint32_t lds, int k, int last, int i, int wave) const {
+    const int first = min(k * kK, last);
+    const uint32_t off = (uint32_t)min(row_[i], last - first) * (uint32_t)ld2 + seg8[i];
+    copy1k(lds + (wave + kWaves * i) * 1024, base + first * ld2, off);
+  }
+  // byte offset of the lane's four values of reduction row 0 of sub-step 0, column block col0
+  __device__ __forceinline__ static int read_at(int col0, int lane) {
+    const int r = (lane & 15) >> 2, row = 4 * (lane >> 5) + r;
+    const int seg = (col0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1) + rot(r)) % SEGS;
+    return row * (COLS * 2) + seg * 16 + (lane & 1) * 8;
+  }
+  __device__ __forceinline__ static u32x4 read(const char* s, int at, int kk) {
+    const char* p = s + at + kk * 16 * (COLS * 2);
+    const u32x2 a = read_tr(p), b = read_tr(p + 8 * (COLS * 2));
+    return (u32x4){a[0], a[1], b[0], b[1]};
+  }
+};
+
+// The exponentials' fragments: 1 KB blocks [half][32 rows][8 columns] of 32 rows x 16 columns, a
+// lane (half h, row r) holding columns 4 h .. + 3 and 8 + 4 h .. + 3.  This is both what a lane of
+// the logits product holds after it, and the operand of dh with the reduction over the
+// vocabulary: no transposition anywhere.
+
+// Runs a workgroup's `tiles` tiles of `steps` reduction steps.  P: the operands.
+//   enter(q)           copies from now on are of tile q
+//   copy(stage, k, c)  copy c of P::NCP of reduction step k
+//   first(s, kk, j), second(s, kk, i): fragments of sub-step kk of the stage at s
+//   fix(f, i)          applied to second's fragment before its products
+//   done(q, acc)       tile q's sums; acc[i][j] = first_j x second_i
+// Sub-step order, copies and barriers: a step's last sub-step is multiplied behind the barrier
+// that ends it, over the next step's first reads; the stage that this barrier frees takes the
+// copies of the step after P::NS, spread over that sub-step and the next two.
+template <typename T, int TM, int TN, typename P>
+__device__ __forceinline__ void stream_tiles(P& p, char* smem, int tiles, int steps) {
+  constexpr int NS = P::NS, NCP = P::NCP, NRD = TM + TN, NMF = TM * TN;
+  float16_t acc[TM][TN];
+  u32x4 f1[2][TN], f2[2][TM];
+  int ct = 0, ck = 0, cstage = 0;  // the copies' tile, step and stage
+  const uint32_t lds0 = lds_addr(smem);
+  auto advance = [&]() {  // to the next step; the last one is copied again rather than none
+    cstage = cstage + 1 == NS ? 0 : cstage + 1;
+    if (ck + 1 < steps) ck++;
+    else if (ct + 1 < tiles) {
+      ct++;
+      ck = 0;
+      p.enter(ct);
+    }
+  };
+  p.enter(0);
+#pragma unroll
+  for (int s = 0; s < NS; s++) {
+#pragma unroll
+    for (int c = 0; c < (s + 1 < NS ? NCP : NCP / 3); c++) p.copy(lds0 + cstage * P::STAGE, ck, c);
+    if (s + 1 < NS) advance();
+  }
+  wait_vmcnt<(NS - 2) * NCP + NCP / 3>();
+  lds_barrier();
+  auto read = [&](int set, const char* s, int kk, int e) {
+    if (e == 0 || e > TN) {
+      const int i = e == 0 ? 0 : e - TN;
+      f2[set][i] = p.second(s, kk, i);
+    } else {
+      f1[set][e - 1] = p.first(s, kk, e - 1);
+    }
+  };
+#pragma unroll
+  for (int e = 0; e < NRD; e++) read(0, smem, 0, e);
+  // multiply set `set`; read sub-step kk of the stage at s into the other one; third `part` of the
+  // copies of the copies' step
+  auto sub = [&](int set, const char* s, int kk, int part) {
+    const int c0 = part < 0 ? 0 : part * NCP / 3, c1 = part < 0 ? 0 : (part + 1) * NCP / 3;
+    int c = c0;
+#pragma unroll
+    for (int i = 0; i < TM; i++) p.fix(f2[set][i], i);
+#pragma unroll
+    for (int e = 0; e < NMF; e++) {
+      const int i = e / TN, j = e % TN;
+      acc[i][j] = Elem<T>::mma(f1[set][j], f2[set][i], acc[i][j]);
+#pragma unroll
+      for (int q = e * NRD / NMF; q < (e + 1) * NRD / NMF; q++) read(set ^ 1, s, kk, q);
+#pragma unroll
+      for (; c < c1 && (e + 1) * (c1 - c0) >= (c - c0 + 1) * NMF; c++)
+        p.copy(lds0 + cstage * P::STAGE, ck, c);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  int stage = 0;
+  for (int q = 0; q < tiles; q++) {
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
+    for (int k = 0; k < steps; k++) {
+      const char* s = smem + stage * P::STAGE;
+      p.step(q, k);
+      sub(0, s, 1, 1);
+      sub(1, s, 2, 2);
+      advance();
+      sub(0, s, 3, -1);
+      wait_vmcnt<(NS - 2) * NCP>();
+      lds_barrier();
+      stage = stage + 1 == NS ? 0 : stage + 1;
+      sub(1, smem + stage * P::STAGE, 0, 0);
+    }
+    p.done(q, acc);
+  }
+  wait_vmem_all();  // no copy may land after the workgroup's end
+}
+
+// ---- logits -----------------------------------------------------------------------------------
+
+// BM rows x kVocabTile columns a tile, WM x (8 / WM) waves.
+template <typename T, int BM, int WM, int NS_, bool KEEP>
+struct Logits {
+  static constexpr int BN = kVocabTile, WN = kWaves / WM, NS = NS_;
+  static constexpr int TM = BM / 32 / WM, TN = BN / 32 / WN;
+  static constexpr int COLS = 32 * TN;  // columns of a wave: one block of statistics
+  using A = RowTile<BM>;
+  using B = RowTile<BN>;
+  static constexpr int STAGE = A::BYTES + B::BYTES, NCP = A::N + B::N;
+  const CeArgs& a;
+  A ca;
+  B cb;
+  int wave, lane, rows, mt, seq0, seqs, wm0, wn0;
+
+  __device__ __forceinline__ Logits(const CeArgs& args) : a(args) {
+    wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    lane = threadIdx.x & 63;
+    wm0 = wave / WN * (BM / WM);
+    wn0 = wave % WN * COLS;
+  }
+  // Tiles in an order that keeps an XCD's 32 workgroups on few operands: groups of four vocabulary
+  // tiles, all row tiles of a group one after the other.  The hardware deals workgroups to the
+  // XCDs in turn, so the 32 of one take consecutive tiles.  Places past the vocabulary are empty.
+  __device__ __forceinline__ int place(int q) const {
+    const int g = (int)gridDim.x, per = g / 8;
+    const int wg = g % 8 ? (int)blockIdx.x : (int)blockIdx.x % 8 * per + (int)blockIdx.x / 8;
+    return q * g + wg;
+  }
+  __device__ __forceinline__ void coords(int at, int& vt, int& m) const {
+    const int g = at / (4 * mt), rest = at - g * 4 * mt;
+    vt = g * 4 + (rest & 3);
+    m = rest >> 2;
+  }
+  __device__ __forceinline__ void enter(int q) {
+    int vt, m;
+    coords(place(q), vt, m);
+    const int last = a.V - 1, v0 = min(vt * BN, last);
+    ca.tile(a.hc, a.D, a.row0 + m * BM, a.row0 + a.rows - 1, wave, lane);
+    cb.tile(a.w, a.ldw, v0, last, wave, lane);
+  }
+  __device__ __forceinline__ void copy(uint32_t lds, int k, int c) const {
+    if (c < A::N) ca.copy(lds, k, c, wave);
+    else cb.copy(lds + A::BYTES, k, c - A::N, wave);
+  }
+  __device__ __forceinline__ u32x4 first(const char* s, int kk, int j) const {
+    return B::read(s + A::BYTES, wn0 + 32 * j, kk, lane);
+  }
+  __device__ __forceinline__ u32x4 second(const char* s, int kk, int i) const {
+    return A::read(s, wm0 + 32 * i, kk, lane);
+  }
+  __device__ __forceinline__ void fix(u32x4&, int) const {}
+  __device__ __forceinline__ void step(int, int) const {}
+
+  // acc[i][j][r]: row 32 i + lane % 32, column 32 j + 8 (r / 4) + 4 (lane / 32) + r % 4.
+  __device__ __forceinline__ void done(int q, float16_t (&acc)[TM][TN]) const {
+    int vt, m;
+    coords(place(q), vt, m);
+    const int v0 = vt * BN + wn0;
+    if (vt * BN >= a.V) return;
+    const int h = lane >> 5;
+    if (v0 + COLS > a.V) {  // columns past the vocabulary
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const bool out = v0 + 32 * j + 8 * (r >> 2) + 4 * h + (r & 3) >= a.V;
+#pragma unroll
+          for (int i = 0; i < TM; i++)
+            if (out) acc[i][j][r] = -__builtin_inff();
+        }
+    }
+    constexpr float kLog2e = 1.44269504088896340736f;
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+      const int row = m * BM + wm0 + 32 * i + (lane & 31);  // of the piece
+      const int y = a.lab[a.row0 + row] - v0;  // the label's column of this wave
+      float top = acc[i][0][0];
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) top = fmaxf(top, acc[i][j][r]);
+      top = fmaxf(top, __shfl_xor(top, 32));
+      // a whole power of two, finite also where every column is -inf
+      top = fmaxf(ceilf(top * kLog2e), -3e38f);
+      const float bias = Elem<T>::kExpBits - top;
+      float sum = 0.0f;
+      if (__any(y >= 0 && y < COLS)) {  // the label's logit goes to zy, its exponential only
+#pragma unroll                          // into the sum
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+          for (int r = 0; r < 16; r++)
+            if (y == 32 * j + 8 * (r >> 2) + 4 * h + (r & 3)) {
+              a.zy[a.row0 + row] = acc[i][j][r];
+              sum = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, bias));
+              acc[i][j][r] = -__builtin_inff();
+            }
+      }
+      u32x4* e = nullptr;
+      if constexpr (KEEP)
+        e = a.e + ((int64_t)(v0 / kK) * (a.rows / 32) + (row >> 5)) * 256 + lane;
+#pragma unroll
+      for (int j = 0; j < TN; j++) {
+        u32x4 f[2];
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, bias));
+          const float z = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r + 1], kLog2e, bias));
+          sum += x;
+          sum += z;
+          if constexpr (KEEP) f[r >> 3][(r & 7) >> 1] = Elem<T>::pack(x, z);
+        }
+        if constexpr (KEEP) {
+          u32x4* to = e + (int64_t)((v0 % kK + 32 * j) / kK) * (a.rows / 32) * 256 +
+                      (v0 % kK + 32 * j) % kK / 16 * 64;
+          to[0] = f[0];
+          to[64] = f[1];
+        }
+      }
+      sum += __shfl_xor(sum, 32);
+      if (h == 0) a.stat[(int64_t)(v0 / COLS) * a.rows + row] = make_float2(top, sum);
+    }
+  }
+};
+
+template <typename T, int BM, int WM, int NS, bool KEEP>
+__global__ __launch_bounds__(kThreads) void k_ce_logits(CeArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  using P = Logits<T, BM, WM, NS, KEEP>;
+  P p(a);
+  p.mt = (piece_rows(a) + BM - 1) / BM;
+  const int vt = (a.V + P::BN - 1) / P::BN, places = (vt + 3) / 4 * 4 * p.mt;
+  const int g = (int)gridDim.x, wg = p.place(0);
+  const int tiles = wg < places ? (places - wg + g - 1) / g : 0;
+  if (tiles > 0) stream_tiles<T, P::TM, P::TN>(p, smem, tiles, a.D / kK);
+}
+
+// ---- statistics of a row ----------------------------------------------------------------------
+
+// Joins the blocks' powers of two and sums.  32 rows x 32 strips of blocks a workgroup.
+template <typename T>
+__global__ __launch_bounds__(1024) void k_ce_join(CeArgs a) {
+  __shared__ float s_top[32][33], s_sum[32][33];
+  const int n = piece_rows(a), r = threadIdx.x & 31, strip = threadIdx.x >> 5;
+  if ((int)blockIdx.x * 32 >= n) return;
+  const int row = (int)blockIdx.x * 32 + r, blocks = (a.V + a.stat_cols - 1) / a.stat_cols;
+  float top = -3e38f, sum = 0.0f;
+  for (int b = strip; b < blocks; b += 32) {
+    const float2 x = a.stat[(int64_t)b * a.rows + row];
+    const float to = fmaxf(top, x.x);
+    sum = sum * __builtin_amdgcn_exp2f(top - to) + x.y * __builtin_amdgcn_exp2f(x.x - to);
+    top = to;
+  }
+  s_top[r][strip] = top;
+  s_sum[r][strip] = sum;
+  __syncthreads();
+  if (strip) return;
+  float to = top;
+  for (int k = 1; k < 32; k++) to = fmaxf(to, s_top[r][k]);
+  sum = 0.0f;
+  for (int k = 0; k < 32; k++) sum += s_sum[r][k] * __builtin_amdgcn_exp2f(s_top[r][k] - to);
+  if (row >= n) return;
+  // the sums are of exponentials times 2^kExpBits
+  sum *= __builtin_amdgcn_exp2f(-Elem<T>::kExpBits);
+  constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+  const int g = a.row0 + row, y = a.lab[g];
+  float loss = __builtin_nanf("");
+  if (y >= 0) {
+    const float d = __builtin_fmaf(a.zy[g], kLog2e, -to);
+    loss = kLn2 * (log2f(sum) - d);
+    loss = loss < 0.0f ? 0.0f : loss;  // rounding; a NaN stays one
+  }
+  RowStat st;
+  st.top = to;
+  st.inv = 1.0f / sum;
+  st.miss = -expm1f(-loss);
+  st.loss = loss;
+  a.row[g] = st;
+  if (a.per_row && a.loss) a.loss[a.idx[g]] = loss;
+}
+
+__global__ __launch_bounds__(1024) void k_ce_loss(CeArgs a) {
+  __shared__ double s[1024];
+  const int t = threadIdx.x, n = a.count[0];
+  double x = 0.0;
+  for (int i = t; i < n; i += 1024) x += (double)a.row[i].loss;
+  s[t] = x;
+  __syncthreads();
+  for (int o = 512; o; o >>= 1) {
+    if (t < o) s[t] += s[t + o];
+    __syncthreads();
+  }
+  if (t == 0) a.loss[0] = (float)(a.mean ? s[0] / (double)n : s[0]);  // 0 / 0 without labels
+}
+
+// ---- dz ---------------------------------------------------------------------------------------
+
+// Exponentials -> dz times 2^kGradBits (and row_grad over its largest magnitude), in place: 32
+// bytes of traffic per eight values.  Rows behind the last become zeros.
+template <typename T>
+__global__ __launch_bounds__(256) void k_ce_dz(CeArgs a) {
+  const int n = piece_rows(a), tbs = a.rows / 32, live = (n + 255) / 256 * 8;
+  const int lane = threadIdx.x & 63, kk = threadIdx.x >> 6, tb = (int)blockIdx.x;
+  if (tb >= live) return;
+  const int row = tb * 32 + (lane & 31), h = lane >> 5, g = a.row0 + row;
+  float f = 0.0f, top = 0.0f, at_label = 0.0f;
+  int y = -1;
+  if (row < n) {
+    const RowStat st = a.row[g];
+    float scale = __builtin_amdgcn_exp2f(Elem<T>::kGradBits);
+    if (a.row_grad)
+      scale = a.gmax[0] != 0.0f ? scale * (a.row_grad[a.idx[g]] / a.gmax[0]) : 0.0f;
+    y = a.lab[g];
+    if (y < 0) scale = __builtin_nanf("");
+    f = st.inv * scale;
+    at_label = -st.miss * scale;
+    top = st.top;
+  }
+  const int steps = (a.V + kVocabTile - 1) / kVocabTile * (kVocabTile / kK);
+  for (int s = (int)blockIdx.y; s < steps; s += (int)gridDim.y) {
+    const int v0 = s * kK + kk * 16;
+    u32x4* p = a.e + ((int64_t)s * tbs + tb) * 256 + threadIdx.x;
+    u32x4 x = *p;
+    float w = 0.0f;
+    if (row < n && v0 < a.V)
+      w = f * __builtin_amdgcn_exp2f(
+                  a.stat[(int64_t)(v0 / a.stat_cols) * a.rows + row].x - top -
+                  Elem<T>::kExpBits);
+    typedef T vec8 __attribute__((ext_vector_type(8)));
+    const vec8 e = __builtin_bit_cast(vec8, x);
+#pragma unroll
+    for (int r = 0; r < 8; r += 2) {
+      float lo = 0.0f, hi = 0.0f;
+      if (row < n) {
+        const int v = v0 + 8 * (r >> 2) + 4 * h + (r & 3);
+        lo = v == y ? at_label : (float)e[r] * w;
+        hi = v + 1 == y ? at_label : (float)e[r + 1] * w;
+      }
+      x[r >> 1] = Elem<T>::pack(lo, hi);
+    }
+    *p = x;
+  }
+}
+
+// ---- dh ---------------------------------------------------------------------------------------
+
+// part[z] [rows, D] = dz W over the z-th share of the vocabulary.
+template <typename T, int BM, int BN, int WM, int NS_>
+struct HiddenGrad {
+  static constexpr int WN = kWaves / WM, NS = NS_, TM = BM / 32 / WM, TN = BN / 32 / WN;
+  using B = ColTile<BN>;
+  static constexpr int A_BYTES = BM * kK * 2, NA = BM / 64;
+  static constexpr int STAGE = A_BYTES + B::BYTES, NCP = NA + B::N;
+  const CeArgs& a;
+  B cb;
+  const char* ebase;
+  int wave, lane, m0, n0, k0, wm0, wn0;
+  int at[TN];
+
+  __device__ __forceinline__ HiddenGrad(const CeArgs& args) : a(args) {
+    wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    lane = threadIdx.x & 63;
+    wm0 = wave / WN * (BM / WM);
+    wn0 = wave % WN * (BN / WN);
+#pragma unroll
+    for (int j = 0; j < TN; j++) at[j] = B::read_at(wn0 + 32 * j, lane);
+  }
+  __device__ __forceinline__ void enter(int) {
+    cb.tile(a.w, a.ldw, n0, a.D, wave, lane);
+    ebase = reinterpret_cast<const char*>(a.e) + (int64_t)(m0 / 32) * 4096;
+  }
+  __device__ __forceinline__ void copy(uint32_t lds, int k, int c) const {
+    if (c < NA) {
+      const int blk = wave * NA + c;
+      copy1k(lds + blk * 1024,
+             ebase + (int64_t)(k0 + k) * (a.rows / 32) * 4096 + blk * 1024, lane * 16);
+    } else {
+      cb.copy(lds + A_BYTES, k0 + k, a.V - 1, c - NA, wave);
+    }
+  }
+  __device__ __forceinline__ u32x4 first(const char* s, int kk, int j) const {
+    return B::read(s + A_BYTES, at[j], kk);
+  }
+  __device__ __forceinline__ u32x4 second(const char* s, int kk, int i) const {
+    return *reinterpret_cast<const u32x4*>(s + (wm0 / 32 + i) * 4096 + kk * 1024 + lane * 16);
+  }
+  __device__ __forceinline__ void fix(u32x4&, int) const {}
+  __device__ __forceinline__ void step(int, int) const {}
+  __device__ __forceinline__ void done(int, float16_t (&acc)[TM][TN]) const {
+    float* out = a.part + (int64_t)blockIdx.z * a.rows * a.D;
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+      float* row = out + (int64_t)(m0 + wm0 + 32 * i + (lane & 31)) * a.D;
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          const int d = n0 + wn0 + 32 * j + 8 * g + 4 * (lane >> 5);
+          if (d < a.D)
+            *reinterpret_cast<float4_t*>(row + d) =
+                (float4_t){acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2],
+                           acc[i][j][4 * g + 3]};
+        }
+    }
+  }
+};
+
+template <typename T, int BM, int BN, int WM, int NS>
+__global__ __launch_bounds__(kThreads) void k_ce_dh(CeArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  using P = HiddenGrad<T, BM, BN, WM, NS>;
+  P p(a);
+  p.m0 = (int)blockIdx.y * BM;
+  p.n0 = (int)blockIdx.x * BN;
+  p.k0 = (int)blockIdx.z * a.split_steps;
+  const int steps = min((a.V + kK - 1) / kK - p.k0, a.split_steps);
+  if (p.m0 < piece_rows(a)) stream_tiles<T, P::TM, P::TN>(p, smem, 1, steps);
+}
+
+// dh rows = the shares' sum, with the scales, to their places in [T, D].
+template <typename T>
+__global__ __launch_bounds__(256) void k_ce_dh_sum(CeArgs a) {
+  const int n = piece_rows(a), row = (int)blockIdx.y;
+  const int d = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 4;
+  if (row >= n || d >= a.D) return;
+  float4_t x = {0, 0, 0, 0};
+  const float* p = a.part + (int64_t)row * a.D + d;
+  for (int z = 0; z < a.splits; z++)
+    x += *reinterpret_cast<const float4_t*>(p + (int64_t)z * a.rows * a.D);
+  float f = __builtin_amdgcn_exp2f(-Elem<T>::kGradBits);
+  if (a.row_grad) f *= a.gmax[0];
+  if (a.mean) f /= (float)a.count[0];
+#pragma unroll
+  for (int e = 0; e < 4; e++) x[e] *= f;
+  *reinterpret_cast<float4_t*>(a.dh + (int64_t)a.idx[a.row0 + row] * a.D + d) = x;
+}
+
+// ---- dW ---------------------------------------------------------------------------------------
+
+// dW [V, D] (+)= dz^T h over the piece's rows: 256 table rows x BN columns a tile.  Both operands
+// have the reduction (the rows of h) across their LDS rows: transposing reads.  A block of dz holds
+// 32 rows; in LDS, row t of half b of column block c lies at place t ^ (4 b + 8 (c % 2)), so that
+// the 32 lanes of a read meet all banks.
+template <typename T, int BN, int NS_>
+struct TableGrad {
+  static constexpr int BM = 256, WM = 4, WN = 2, NS = NS_, TM = 2, TN = BN / 64;
+  using B = ColTile<BN>;
+  static constexpr int A_BYTES = BM * kK * 2, NA = 4;
+  static constexpr int STAGE = A_BYTES + B::BYTES, NCP = NA + B::N;
+  const CeArgs& a;
+  B cb;
+  const char* ebase;
+  int wave, lane, nt, n0, wm0, wn0;
+  int at[TN], eat[2][2];
+
+  __device__ __forceinline__ TableGrad(const CeArgs& args) : a(args) {
+    wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    lane = threadIdx.x & 63;
+    wm0 = wave / WN * 64;
+    wn0 = wave % WN * (BN / WN);
+#pragma unroll
+    for (int j = 0; j < TN; j++) at[j] = B::read_at(wn0 + 32 * j, lane);
+    const int r = (lane & 15) >> 2, s = lane & 3, c = (lane >> 4) & 1, b = s & 1;
+#pragma unroll
+    for (int odd = 0; odd < 2; odd++)  // sub-step's parity: rows 16 odd .. of a block
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        const int t = 16 * odd + 8 * x + 4 * (lane >> 5) + r;
+        eat[odd][x] = c * 1024 + b * 512 + (t ^ (4 * b + 8 * c)) * 16 + (s >> 1) * 8;
+      }
+  }
+  __device__ __forceinline__ int place(int q) const { return q * (int)gridDim.x + (int)blockIdx.x; }
+  __device__ __forceinline__ void coords(int q, int& v, int& n) const {
+    const int at = place(q);
+    v = at / nt;
+    n = at - v * nt;
+  }
+  __device__ __forceinline__ void enter(int q) {
+    int v, n;
+    coords(q, v, n);
+    cb.tile(static_cast<const uint16_t*>(a.hc) + (int64_t)a.row0 * a.D, a.D, n * BN, a.D, wave,
+            lane);
+    ebase = reinterpret_cast<const char*>(a.e) + (int64_t)v * 4 * (a.rows / 32) * 4096;
+  }
+  __device__ __forceinline__ void copy(uint32_t lds, int k, int c) const {
+    if (c < NA) {  // wave: columns 64 (wave / 2) .., rows 32 (wave % 2) ..; c: 16 columns
+      const int swap = 4 * (lane >> 5) + 8 * (c & 1);
+      const uint32_t off = ((lane & 32) + ((lane & 31) ^ swap)) * 16;
+      copy1k(lds + wave * 4096 + c * 1024,
+             ebase + ((int64_t)(wave >> 1) * (a.rows / 32) + 2 * k + (wave & 1)) * 4096 +
+                 c * 1024,
+             off);
+    } else {
+      cb.copy(lds + A_BYTES, k, a.rows - 1, c - NA, wave);
+    }
+  }
+  __device__ __forceinline__ u32x4 first(const char* s, int kk, int j) const {
+    return B::read(s + A_BYTES, at[j], kk);
+  }
+  __device__ __forceinline__ u32x4 second(const char* s, int kk, int i) const {
+    const int block = wm0 / 32 + i;  // 32 table rows: half of a 64-column group
+    const char* p = s + (block >> 1) * 8192 + (kk >> 1) * 4096 + (block & 1) * 2048;
+    const u32x2 x = read_tr(p + eat[kk & 1][0]), y = read_tr(p + eat[kk & 1][1]);
+    return (u32x4){x[0], x[1], y[0], y[1]};
+  }
+  __device__ __forceinline__ void fix(u32x4&, int) const {}
+  __device__ __forceinline__ void step(int, int) const {}
+  __device__ __forceinline__ void done(int q, float16_t (&acc)[TM][TN]) const {
+    int v, n;
+    coords(q, v, n);
+    float f = __builtin_amdgcn_exp2f(-Elem<T>::kGradBits);
+    if (a.row_grad) f *= a.gmax[0];
+    if (a.mean) f /= (float)max(a.count[0], 1);
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+      const int row = v * BM + wm0 + 32 * i + (lane & 31);
+      if (row >= a.V) continue;
+      float* out = a.dw + (int64_t)row * a.D;
+#pragma unroll
+      for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          const int d = n * BN + wn0 + 32 * j + 8 * g + 4 * (lane >> 5);
+          if (d >= a.D) continue;
+          float4_t x;
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[e] = acc[i][j][4 * g + e] * f;
+          if (!a.first) x += *reinterpret_cast<const float4_t*>(out + d);
+          *reinterpret_cast<float4_t*>(out + d) = x;
+        }
+    }
+  }
+};
+
+template <typename T, int BN, int NS>
+__global__ __launch_bounds__(kThreads) void k_ce_dw(CeArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  using P = TableGrad<T, BN, NS>;
+  P p(a);
+  p.nt = (a.D + BN - 1) / BN;
+  const int places = (a.V + P::BM - 1) / P::BM * p.nt, g = (int)gridDim.x;
+  const int wg = (int)blockIdx.x, tiles = wg < places ? (places - wg + g - 1) / g : 0;
+  const int steps = (piece_rows(a) + kK - 1) / kK;
+  if (tiles == 0) return;
+  if (steps > 0) {
+    stream_tiles<T, P::TM, P::TN>(p, smem, tiles, steps);
+  } else if (a.first) {  // no row has a label
+    float16_t acc[P::TM][P::TN] = {};
+    for (int q = 0; q < tiles; q++) p.done(q, acc);
+  }
+}
+
+// ---- gradients to their type --------------------------------------------------------------------
+
+// out = unit * g (one value, or one per row), rounded once.
+template <typename T>
+__global__ __launch_bounds__(256) void k_ce_scale(const float* unit, const float* g, int per_row,
+                                                  int64_t chunks, int row_chunks, T* out) {
+  typedef T vec8 __attribute__((ext_vector_type(8)));
+  for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < chunks;
+       c += (int64_t)gridDim.x * 256) {
+    const float f = g[per_row ? c / row_chunks : 0];
+    const float4_t x = reinterpret_cast<const float4_t*>(unit)[2 * c];
+    const float4_t y = reinterpret_cast<const float4_t*>(unit)[2 * c + 1];
+    vec8 o;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      o[e] = (T)(x[e] * f);
+      o[4 + e] = (T)(y[e] * f);
+    }
+    reinterpret_cast<vec8*>(out)[c] = o;
+  }
+}
+
+// ---- host side --------------------------------------------------------------------------------
+
+static int ce_launched() {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? MXS_OK : (int)e;
+}
+
+// Compute units of the current device (its workgroups fill them one each).
+static int ce_cus() {
+  static int counts[16];
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 16) return 256;
+  if (counts[dev] == 0) {
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+        n <= 0)
+      n = 256;
+    counts[dev] = n;
+  }
+  return counts[dev];
+}
+
+template <typename K>
+static int ce_lds(K fn, int bytes, bool (&set)[16]) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) dev = -1;
+  if (dev >= 0 && dev < 16 && set[dev]) return MXS_OK;  // idempotent: a benign race
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return (int)e;
+  if (dev >= 0 && dev < 16) set[dev] = true;
+  return MXS_OK;
+}
+
+// How a call runs: pieces of the rows, tiles and shares.
+struct CePlan {
+  int Tp, rows, pieces;   // padded rows, rows of a piece
+  int bm;                 // rows of a logits tile: 256, 128, 64 or 32
+  int stat_cols, blocks;
+  int dh_bm, dh_bn, splits, split_steps;
+  int64_t vp;             // vocabulary in whole tiles
+};
+
+static CePlan ce_plan(int T, int V, int D, bool grads, int cus) {
+  CePlan p;
+  p.Tp = (T + kRowPad - 1) / kRowPad * kRowPad;
+  p.vp = (int64_t)((V + kVocabTile - 1) / kVocabTile) * kVocabTile;
+  int64_t most = kRowPad;
+  if (grads)
+    while (2 * most * p.vp * 2 <= kPieceBytes && most < p.Tp) most *= 2;
+  else
+    while (most < p.Tp && most < 8192) most *= 2;  // 8 KB of statistics a row at 128 K columns
+  p.pieces = (int)((p.Tp + most - 1) / most);
+  p.rows = (int)((p.Tp / kRowPad + p.pieces - 1) / p.pieces) * kRowPad;
+  p.bm = T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
+  p.stat_cols = p.bm == 256 ? 128 : p.bm == 32 ? 32 : 64;
+  p.blocks = (int)(p.vp / p.stat_cols);
+  p.dh_bm = T <= 64 ? 64 : 256;
+  const int steps = (V + kK - 1) / kK;
+  const int mt = ((p.pieces > 1 ? p.rows : T) + p.dh_bm - 1) / p.dh_bm;
+  double best = 0;
+  for (int bn : {256, 192, 128}) {
+    if (bn == 192 && p.dh_bm == 64) continue;  // six column blocks do not share out over the waves
+    const int tiles = mt * ((D + bn - 1) / bn);
+    for (int s = 1; s <= 64 && s <= (steps + 7) / 8; s++) {
+      const int per = (steps + s - 1) / s, z = (steps + per - 1) / per;
+      const int rounds = (tiles * z + cus - 1) / cus;
+      // a step's cost by its tile's width, the shares' sums as traffic
+      const double cost = rounds * (per * (0.25 + bn / 256.0) + 12) + 0.25 * z * mt;
+      if (best == 0 || cost < best) {
+        best = cost;
+        p.dh_bn = bn;
+        p.splits = z;
+        p.split_steps = per;
+      }
+    }
+  }
+  return p;
+}
+
+struct CeLayout {
+  int64_t idx, lab, hc, row, zy, stat, e, part, end;
+};
+
+static CeLayout ce_layout(const CePlan& p, int D, bool grads, bool dh) {
+  CeLayout l;
+  int64_t at = 256;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += (bytes + 255) / 256 * 256;
+    return o;
+  };
+  l.idx = take(4LL * p.Tp);
+  l.lab = take(4LL * p.Tp);
+  l.hc = take(2LL * p.Tp * D);
+  l.row = take(16LL * p.Tp);
+  l.zy = take(4LL * p.Tp);
+  l.stat = take(8LL * p.blocks * p.rows);
+  l.e = grads ? take(2LL * p.vp * p.rows) : 0;
+  l.part = dh ? take(4LL * p.splits * p.rows * D) : 0;
+  l.end = at;
+  return l;
+}
+
+template <typename T, int BM, int WM, int NS, bool KEEP>
+static int launch_logits(const CeArgs& a, int cus, hipStream_t stream) {
+  using P = Logits<T, BM, WM, NS, KEEP>;
+  static bool set[16];
+  auto* fn = &k_ce_logits<T, BM, WM, NS, KEEP>;
+  const int rc = ce_lds(fn, NS * P::STAGE, set);
+  if (rc != MXS_OK) return rc;
+  const int per_cu = 2 * NS * P::STAGE <= 160 * 1024 ? 2 : 1;
+  hipLaunchKernelGGL(fn, dim3(cus * per_cu), dim3(kThreads), NS * P::STAGE, stream, a);
+  return ce_launched();
+}
+
+template <typename T, int BM, int BN, int WM, int NS>
+static int launch_dh(const CeArgs& a, const CePlan& p, hipStream_t stream) {
+  using P = HiddenGrad<T, BM, BN, WM, NS>;
+  static bool set[16];
+  auto* fn = &k_ce_dh<T, BM, BN, WM, NS>;
+  const int rc = ce_lds(fn, NS * P::STAGE, set);
+  if (rc != MXS_OK) return rc;
+  const int rows = a.rows < a.T ? a.rows : a.T;
+  hipLaunchKernelGGL(fn, dim3((a.D + BN - 1) / BN, (rows + BM - 1) / BM, p.splits),
+                     dim3(kThreads), NS * P::STAGE, stream, a);
+  return ce_launched();
+}
+
+template <typename T, int BN, int NS>
+static int launch_dw(const CeArgs& a, int cus, hipStream_t stream) {
+  using P = TableGrad<T, BN, NS>;
+  static bool set[16];
+  auto* fn = &k_ce_dw<T, BN, NS>;
+  const int rc = ce_lds(fn, NS * P::STAGE, set);
+  if (rc != MXS_OK) return rc;
+  hipLaunchKernelGGL(fn, dim3(cus), dim3(kThreads), NS * P::STAGE, stream, a);
+  return ce_launched();
+}
+
+#define CE_TRY(call)                      \
+  do {                                    \
+    const int rc_ = (call);               \
+    if (rc_ != MXS_OK) return rc_;        \
+  } while (0)
+
+template <typename T, bool KEEP>
+static int logits_of(const CeArgs& a, const CePlan& p, int cus, hipStream_t stream) {
+  switch (p.bm) {
+    case 32: return launch_logits<T, 32, 1, 4, KEEP>(a, cus, stream);
+    case 64: return launch_logits<T, 64, 2, 3, KEEP>(a, cus, stream);
+    case 128: return launch_logits<T, 128, 2, 3, KEEP>(a, cus, stream);
+    default: return launch_logits<T, 256, 4, 2, KEEP>(a, cus, stream);
+  }
+}
+
+template <typename T>
+static int dh_of(const CeArgs& a, const CePlan& p, hipStream_t stream) {
+  if (p.dh_bm == 64) {
+    switch (p.dh_bn) {
+      case 256: return launch_dh<T, 64, 256, 2, 3>(a, p, stream);
+      default: return launch_dh<T, 64, 128, 2, 3>(a, p, stream);
+    }
+  }
+  switch (p.dh_bn) {
+    case 256: return launch_dh<T, 256, 256, 4, 2>(a, p, stream);
+    case 192: return launch_dh<T, 256, 192, 4, 2>(a, p, stream);
+    default: return launch_dh<T, 256, 128, 4, 3>(a, p, stream);
+  }
+}
+
+template <typename T>
+static int run_ce(CeArgs a, const CePlan& p, int cus, hipStream_t stream) {
+  const bool grads = a.dh || a.dw;
+  const int vec = (uintptr_t)a.h % 16 == 0 && a.ldh % 8 == 0;
+  hipLaunchKernelGGL(k_ce_rows, dim3(p.Tp / kGather), dim3(256), 0, stream, a, vec);
+  CE_TRY(ce_launched());
+  if (grads && a.row_grad) {
+    hipLaunchKernelGGL(k_ce_gmax, dim3(1), dim3(1024), 0, stream, a);
+    CE_TRY(ce_launched());
+  }
+  for (int i = 0; i < p.pieces; i++) {
+    a.row0 = i * p.rows;
+    a.rows = p.rows < p.Tp - a.row0 ? p.rows : p.Tp - a.row0;
+    a.first = i == 0;
+    CE_TRY(grads ? (logits_of<T, true>(a, p, cus, stream))
+                 : (logits_of<T, false>(a, p, cus, stream)));
+    hipLaunchKernelGGL(k_ce_join<T>, dim3(a.rows / 32), dim3(1024), 0, stream, a);
+    CE_TRY(ce_launched());
+    if (!grads) continue;
+    const int tbs = a.rows / 32, ys = 4096 / tbs + 1;
+    hipLaunchKernelGGL(k_ce_dz<T>, dim3(tbs, ys), dim3(256), 0, stream, a);
+    CE_TRY(ce_launched());
+    if (a.dh) {
+      CE_TRY(dh_of<T>(a, p, stream));
+      hipLaunchKernelGGL(k_ce_dh_sum<T>, dim3((a.D / 4 + 255) / 256, a.rows), dim3(256), 0,
+                         stream, a);
+      CE_TRY(ce_launched());
+    }
+    if (a.dw) CE_TRY((launch_dw<T, 256, 2>(a, cus, stream)));
+  }
+  if (a.loss && !a.per_row) {
+    hipLaunchKernelGGL(k_ce_loss, dim3(1), dim3(1024), 0, stream, a);
+    CE_TRY(ce_launched());
+  }
+  return MXS_OK;
+}
+
+static int ce_sizes(int T, int V, int D) {
+  if (T < 0 || V <= 0 || D <= 0) return MXS_ERR_ARG;
+  return D % kK || D > 65536 || T > (1 << 24) || V > (1 << 28) ? MXS_ERR_SIZE : MXS_OK;
+}
+
+}  // namespace mxs
+
+using namespace mxs;
+
+extern "C" {
+
+int64_t mxs_head_ce_workspace_bytes(int T, int V, int D, int want_dh, int want_dw) {
+  const int rc = ce_sizes(T, V, D);
+  if (rc != MXS_OK) return rc;
+  const bool grads = want_dh || want_dw;
+  return ce_layout(ce_plan(T > 0 ? T : 1, V, D, grads, ce_cus()), D, grads, want_dh != 0).end;
+}
+
+int mxs_head_ce(const void* h, int64_t ldh, const void* w, int64_t ldw, const int64_t* labels,
+                int T, int V, int D, int dtype, int64_t ignore_index, int reduction,
+                const float* row_grad, float* loss, float* dh, float* dw, void* workspace,
+                hipStream_t stream) {
+  const int rc = ce_sizes(T, V, D);
+  if (rc != MXS_OK) return rc;
+  if (dtype != MXS_DTYPE_F16 && dtype != MXS_DTYPE_BF16) return MXS_ERR_DTYPE;
+  if (!w || !workspace || (T && (!h || !labels || (!loss && !dh && !dw))))
+    return MXS_ERR_ARG;
+  if (reduction < 0 || reduction > 2 || ldh < D || ldw < D) return MXS_ERR_ARG;
+  if (T && dw && reduction == 0 && !row_grad) return MXS_ERR_ARG;
+  if ((uintptr_t)w % 16 || ldw % 8 || (uintptr_t)workspace % 256) return MXS_ERR_ALIGN;
+  if ((uintptr_t)dh % 16 || (uintptr_t)dw % 16) return MXS_ERR_ALIGN;
+  // offsets within a tile are 32 bits
+  if (ldw > (1 << 22) || ldh > ((int64_t)1 << 40)) return MXS_ERR_SIZE;
+  const int cus = ce_cus();
+  const bool grads = dh || dw;
+  const CePlan p = ce_plan(T > 0 ? T : 1, V, D, grads, cus);
+  const CeLayout l = ce_layout(p, D, grads, dh != nullptr);
+  char* ws = static_cast<char*>(workspace);
+  CeArgs a = {};
+  a.h = h, a.ldh = ldh, a.w = w, a.ldw = ldw, a.labels = labels, a.ignore = ignore_index;
+  a.T = T, a.V = V, a.D = D, a.row_grad = row_grad, a.loss = loss, a.dh = dh, a.dw = dw;
+  a.per_row = reduction == 0;
+  a.mean = reduction == 2;
+  a.count = reinterpret_cast<int*>(ws);
+  a.gmax = reinterpret_cast<float*>(ws + 4);
+  a.idx = reinterpret_cast<int*>(ws + l.idx);
+  a.lab = reinterpret_cast<int*>(ws + l.lab);
+  a.hc = ws + l.hc;
+  a.row = reinterpret_cast<RowStat*>(ws + l.row);
+  a.zy = reinterpret_cast<float*>(ws + l.zy);
+  a.stat = reinterpret_cast<float2*>(ws + l.stat);
+  a.e = reinterpret_cast<u32x4*>(ws + l.e);
+  a.part = reinterpret_cast<float*>(ws + l.part);
+  a.stat_cols = p.stat_cols;
+  a.splits = p.splits, a.split_steps = p.split_steps;
+  return dtype == MXS_DTYPE_F16 ? run_ce<_Float16>(a, p, cus, stream)
+                                : run_ce<__bf16>(a, p, cus, stream);
+}
+
+int mxs_head_ce_grad(const float* unit, const float* g, int per_row, int64_t rows, int cols,
+                     int dtype, void* out, hipStream_t stream) {
+  if (rows < 0 || cols <= 0) return MXS_ERR_ARG;
+  if (dtype != MXS_DTYPE_F16 && dtype != MXS_DTYPE_BF16) return MXS_ERR_DTYPE;
+  if (cols % 8) return MXS_ERR_SIZE;
+  if (rows == 0) return MXS_OK;
+  if (!unit || !g || !out) return MXS_ERR_ARG;
+  if ((uintptr_t)unit % 16 || (uintptr_t)out % 16) return MXS_ERR_ALIGN;
+  const int64_t chunks = rows * (cols / 8), wgs = (chunks + 255) / 256;
+  const dim3 grid((unsigned)(wgs < 8192 ? wgs : 8192));
+  if (dtype == MXS_DTYPE_F16)
+    hipLaunchKernelGGL(k_ce_scale<_Float16>, grid, dim3(256), 0, stream, unit, g, per_row, chunks,
+                       cols / 8, static_cast<_Float16*>(out));
+  else
+    hipLaunchKernelGGL(k_ce_scale<__bf16>, grid, dim3(256), 0, stream, unit, g, per_row, chunks,
+                       cols / 8, static_cast<__bf16*>(out));
+  return ce_launched();
+}
+
+}  // extern "C"
