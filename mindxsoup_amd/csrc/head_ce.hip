@@ -62,8 +62,8 @@ struct Elem<__bf16> {
 // ---- what the kernels of a call share -----------------------------------------------------------
 
 struct RowStat {
-  float top;    // whole power of two that the row's sum is relative to
-  float inv;    // 1 / sum of 2^(z log2 e - top)
+  float top;    // whole power of two that the row's exponentials but the label's are relative to
+  float inv;    // 1 / sum of 2^(z log2 e - top), the label's included
   float miss;   // 1 - p of the label
   float loss;
 };
@@ -90,6 +90,7 @@ struct CeArgs {
   RowStat* row;      // [Tp]
   float* zy;         // [Tp] the label's logit
   float2* stat;      // [blocks][piece rows] power of two and sum of a block of columns
+  uint32_t* shift;   // [blocks][piece rows] binades from a block's to its row's power of two
   u32x4* e;          // [Vp / 64][piece rows / 32][4][64] fragments of exponentials, then dz
   float* part;       // [splits][piece rows][D]
   // the piece
@@ -105,34 +106,32 @@ __device__ __forceinline__ int piece_rows(const CeArgs& a) {
 
 // ---- rows with a label ------------------------------------------------------------------------
 
-constexpr int kGather = 32;  // gathered rows of a workgroup
+constexpr int kGather = 8;  // gathered rows of a workgroup
 
 // Gathers the rows whose label is not `ignore`, in order, and pads with zeros.  Every workgroup
 // counts all the labels itself (an L2 read of 8 T bytes; one launch, no waiting on another
 // workgroup) and copies its own rows.  Ignored rows get their zeros in loss and dh here.
 __global__ __launch_bounds__(256) void k_ce_rows(CeArgs a, int vec) {
-  __shared__ int s_sum[256], s_idx[kGather];
-  const int t = threadIdx.x, r0 = (int)blockIdx.x * kGather;
-  const int per = (a.T + 255) / 256, t0 = min(t * per, a.T), t1 = min(t0 + per, a.T);
+  __shared__ int s_sum[4], s_idx[kGather];
+  const int t = threadIdx.x, r0 = (int)blockIdx.x * kGather, lane = t & 63, wave = t >> 6;
+  const int seg = (a.T + 255) / 256 * 64, t0 = min(wave * seg, a.T), t1 = min(t0 + seg, a.T);
   int n = 0;
-  for (int i = t0; i < t1; i++) n += a.labels[i] != a.ignore ? 1 : 0;
-  s_sum[t] = n;
+  for (int i = t0; i < t1; i += 64)
+    n += __popcll(__ballot(i + lane < t1 && a.labels[i + lane] != a.ignore));
+  if (lane == 0) s_sum[wave] = n;
   if (t < kGather) s_idx[t] = -1;
   __syncthreads();
-  for (int o = 1; o < 256; o <<= 1) {
-    const int v = t >= o ? s_sum[t - o] : 0;
-    __syncthreads();
-    s_sum[t] += v;
-    __syncthreads();
-  }
-  if (r0 == 0 && t == 0) a.count[0] = s_sum[255];
-  int at = s_sum[t] - n;
+  int at = 0;
+  for (int w = 0; w < wave; w++) at += s_sum[w];
+  if (r0 == 0 && t == 0) a.count[0] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
   if (at < r0 + kGather && at + n > r0)
-    for (int i = t0; i < t1; i++)
-      if (a.labels[i] != a.ignore) {
-        if (at >= r0 && at < r0 + kGather) s_idx[at - r0] = i;
-        at++;
-      }
+    for (int i = t0; i < t1 && at < r0 + kGather; i += 64) {
+      const bool has = i + lane < t1 && a.labels[i + lane] != a.ignore;
+      const uint64_t all = __ballot(has);
+      const int place = at + __popcll(all & ((1ull << lane) - 1));
+      if (has && place >= r0 && place < r0 + kGather) s_idx[place - r0] = i + lane;
+      at += __popcll(all);
+    }
   __syncthreads();
   if (t < kGather) {
     const int i = s_idx[t];
@@ -145,20 +144,24 @@ __global__ __launch_bounds__(256) void k_ce_rows(CeArgs a, int vec) {
     a.lab[r0 + t] = y;
   }
   const int chunks = a.D / 8;  // 16-byte pieces of a row
-  u32x4* out = static_cast<u32x4*>(a.hc) + (int64_t)r0 * chunks;
-  for (int c = t; c < kGather * chunks; c += 256) {
-    const int r = c / chunks, k = c - r * chunks, i = s_idx[r];
-    u32x4 v = {0, 0, 0, 0};
-    if (i >= 0) {
-      const uint16_t* src = static_cast<const uint16_t*>(a.h) + (int64_t)i * a.ldh + 8 * k;
-      if (vec) {
-        v = *reinterpret_cast<const u32x4*>(src);
-      } else {
+  for (int r = wave * 2; r < wave * 2 + 2; r++) {
+    const int i = s_idx[r];
+    u32x4* out = static_cast<u32x4*>(a.hc) + (int64_t)(r0 + r) * chunks;
+    const uint16_t* row = static_cast<const uint16_t*>(a.h) + (int64_t)i * a.ldh;
+#pragma unroll 4
+    for (int k = lane; k < chunks; k += 64) {
+      u32x4 v = {0, 0, 0, 0};
+      if (i >= 0) {
+        const uint16_t* src = row + 8 * k;
+        if (vec) {
+          v = *reinterpret_cast<const u32x4*>(src);
+        } else {
 #pragma unroll
-        for (int q = 0; q < 4; q++) v[q] = src[2 * q] | ((uint32_t)src[2 * q + 1] << 16);
+          for (int q = 0; q < 4; q++) v[q] = src[2 * q] | ((uint32_t)src[2 * q + 1] << 16);
+        }
       }
+      out[k] = v;
     }
-    out[c] = v;
   }
   for (int r = 0; r < kGather; r++) {
     const int i = r0 + r;
@@ -169,6 +172,7 @@ __global__ __launch_bounds__(256) void k_ce_rows(CeArgs a, int vec) {
         reinterpret_cast<float4_t*>(a.dh + (int64_t)i * a.D)[k] = (float4_t){0, 0, 0, 0};
   }
 }
+static_assert(kGather == 8, "two rows a wave");
 
 // Largest |row_grad| of the rows with a label: dz is kept relative to it, in fp16's range.
 __global__ __launch_bounds__(1024) void k_ce_gmax(CeArgs a) {
@@ -306,6 +310,7 @@ struct ColTile {
 //   copy(stage, k, c)  copy c of P::NCP of reduction step k
 //   first(s, kk, j), second(s, kk, i): fragments of sub-step kk of the stage at s
 //   fix(f, i)          applied to second's fragment before its products
+//   load(s), next()    what fix needs of the reduction step in stage s: read, then taken over
 //   done(q, acc)       tile q's sums; acc[i][j] = first_j x second_i
 // Sub-step order, copies and barriers: a step's last sub-step is multiplied behind the barrier
 // that ends it, over the next step's first reads; the stage that this barrier frees takes the
@@ -345,6 +350,8 @@ __device__ __forceinline__ void stream_tiles(P& p, char* smem, int tiles, int st
   };
 #pragma unroll
   for (int e = 0; e < NRD; e++) read(0, smem, 0, e);
+  p.load(smem);
+  p.next();
   // multiply set `set`; read sub-step kk of the stage at s into the other one; third `part` of the
   // copies of the copies' step
   auto sub = [&](int set, const char* s, int kk, int part) {
@@ -374,7 +381,6 @@ __device__ __forceinline__ void stream_tiles(P& p, char* smem, int tiles, int st
         for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
     for (int k = 0; k < steps; k++) {
       const char* s = smem + stage * P::STAGE;
-      p.step(q, k);
       sub(0, s, 1, 1);
       sub(1, s, 2, 2);
       advance();
@@ -382,11 +388,20 @@ __device__ __forceinline__ void stream_tiles(P& p, char* smem, int tiles, int st
       wait_vmcnt<(NS - 2) * NCP>();
       lds_barrier();
       stage = stage + 1 == NS ? 0 : stage + 1;
+      p.load(smem + stage * P::STAGE);
       sub(1, smem + stage * P::STAGE, 0, 0);
+      p.next();
     }
     p.done(q, acc);
   }
   wait_vmem_all();  // no copy may land after the workgroup's end
+}
+
+// Place of workgroup `b` of n in an order in which each XCD (the hardware deals workgroups to the
+// eight of them in turn) takes consecutive places.
+__device__ __forceinline__ int xcd_place(int b, int n) {
+  const int x = b & 7, j = b >> 3, per = n >> 3, rem = n & 7;
+  return x * per + min(x, rem) + j;
 }
 
 // ---- logits -----------------------------------------------------------------------------------
@@ -415,9 +430,7 @@ struct Logits {
   // tiles, all row tiles of a group one after the other.  The hardware deals workgroups to the
   // XCDs in turn, so the 32 of one take consecutive tiles.  Places past the vocabulary are empty.
   __device__ __forceinline__ int place(int q) const {
-    const int g = (int)gridDim.x, per = g / 8;
-    const int wg = g % 8 ? (int)blockIdx.x : (int)blockIdx.x % 8 * per + (int)blockIdx.x / 8;
-    return q * g + wg;
+    return q * (int)gridDim.x + xcd_place((int)blockIdx.x, (int)gridDim.x);
   }
   __device__ __forceinline__ void coords(int at, int& vt, int& m) const {
     const int g = at / (4 * mt), rest = at - g * 4 * mt;
@@ -442,7 +455,8 @@ struct Logits {
     return A::read(s, wm0 + 32 * i, kk, lane);
   }
   __device__ __forceinline__ void fix(u32x4&, int) const {}
-  __device__ __forceinline__ void step(int, int) const {}
+  __device__ __forceinline__ void load(const char*) const {}
+  __device__ __forceinline__ void next() const {}
 
   // acc[i][j][r]: row 32 i + lane % 32, column 32 j + 8 (r / 4) + 4 (lane / 32) + r % 4.
   __device__ __forceinline__ void done(int q, float16_t (&acc)[TM][TN]) const {
@@ -467,6 +481,16 @@ struct Logits {
     for (int i = 0; i < TM; i++) {
       const int row = m * BM + wm0 + 32 * i + (lane & 31);  // of the piece
       const int y = a.lab[a.row0 + row] - v0;  // the label's column of this wave
+      if (__any(y >= 0 && y < COLS)) {  // the label's logit goes to zy alone
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+          for (int r = 0; r < 16; r++)
+            if (y == 32 * j + 8 * (r >> 2) + 4 * h + (r & 3)) {
+              a.zy[a.row0 + row] = acc[i][j][r];
+              acc[i][j][r] = -__builtin_inff();
+            }
+      }
       float top = acc[i][0][0];
 #pragma unroll
       for (int j = 0; j < TN; j++)
@@ -477,17 +501,6 @@ struct Logits {
       top = fmaxf(ceilf(top * kLog2e), -3e38f);
       const float bias = Elem<T>::kExpBits - top;
       float sum = 0.0f;
-      if (__any(y >= 0 && y < COLS)) {  // the label's logit goes to zy, its exponential only
-#pragma unroll                          // into the sum
-        for (int j = 0; j < TN; j++)
-#pragma unroll
-          for (int r = 0; r < 16; r++)
-            if (y == 32 * j + 8 * (r >> 2) + 4 * h + (r & 3)) {
-              a.zy[a.row0 + row] = acc[i][j][r];
-              sum = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, bias));
-              acc[i][j][r] = -__builtin_inff();
-            }
-      }
       u32x4* e = nullptr;
       if constexpr (KEEP)
         e = a.e + ((int64_t)(v0 / kK) * (a.rows / 32) + (row >> 5)) * 256 + lane;
@@ -529,46 +542,61 @@ __global__ __launch_bounds__(kThreads) void k_ce_logits(CeArgs a) {
 
 // ---- statistics of a row ----------------------------------------------------------------------
 
-// Joins the blocks' powers of two and sums.  32 rows x 32 strips of blocks a workgroup.
-template <typename T>
+constexpr int kJoinRows = 8;  // rows of a workgroup, over 128 strips of blocks
+
+// Joins the blocks' powers of two and sums, all but the label's, and with the label's logit gives
+// the row's loss: log(1 + rest / label), which stays exact for a label that is all but certain.
+// SHIFT: leaves each block's distance to the row's power of two for dh, in both halves of a word
+// and at the place of the exponent in a T.
+template <typename T, bool SHIFT>
 __global__ __launch_bounds__(1024) void k_ce_join(CeArgs a) {
-  __shared__ float s_top[32][33], s_sum[32][33];
-  const int n = piece_rows(a), r = threadIdx.x & 31, strip = threadIdx.x >> 5;
-  if ((int)blockIdx.x * 32 >= n) return;
-  const int row = (int)blockIdx.x * 32 + r, blocks = (a.V + a.stat_cols - 1) / a.stat_cols;
+  __shared__ float2 s_part[16][kJoinRows];
+  const int n = piece_rows(a), r = threadIdx.x % kJoinRows, strip = threadIdx.x / kJoinRows;
+  if ((int)blockIdx.x * kJoinRows >= n) return;
+  const int row = (int)blockIdx.x * kJoinRows + r;
+  const int blocks = (a.V + a.stat_cols - 1) / a.stat_cols;
   float top = -3e38f, sum = 0.0f;
-  for (int b = strip; b < blocks; b += 32) {
-    const float2 x = a.stat[(int64_t)b * a.rows + row];
-    const float to = fmaxf(top, x.x);
-    sum = sum * __builtin_amdgcn_exp2f(top - to) + x.y * __builtin_amdgcn_exp2f(x.x - to);
+  auto join = [&](float t, float s) {
+    const float to = fmaxf(top, t);
+    sum = sum * __builtin_amdgcn_exp2f(top - to) + s * __builtin_amdgcn_exp2f(t - to);
     top = to;
+  };
+  constexpr int kStrips = 1024 / kJoinRows;
+#pragma unroll 4
+  for (int b = strip; b < blocks; b += kStrips) {
+    const float2 x = a.stat[(int64_t)b * a.rows + row];
+    join(x.x, x.y);
   }
-  s_top[r][strip] = top;
-  s_sum[r][strip] = sum;
+#pragma unroll
+  for (int o = kJoinRows; o < 64; o <<= 1) join(__shfl_xor(top, o), __shfl_xor(sum, o));
+  if ((threadIdx.x & 63) < kJoinRows) s_part[threadIdx.x >> 6][r] = make_float2(top, sum);
   __syncthreads();
-  if (strip) return;
-  float to = top;
-  for (int k = 1; k < 32; k++) to = fmaxf(to, s_top[r][k]);
-  sum = 0.0f;
-  for (int k = 0; k < 32; k++) sum += s_sum[r][k] * __builtin_amdgcn_exp2f(s_top[r][k] - to);
+  top = -3e38f, sum = 0.0f;
+  for (int w = 0; w < 16; w++) join(s_part[w][r].x, s_part[w][r].y);
   if (row >= n) return;
+  if constexpr (SHIFT) {
+    constexpr int kBits = sizeof(T) == 2 && Elem<T>::kExpBits > 0 ? 10 : 7;
+    constexpr float kMost = kBits == 10 ? 31.0f : 255.0f;
+    for (int b = strip; b < blocks; b += kStrips) {
+      const float d = top - a.stat[(int64_t)b * a.rows + row].x;
+      a.shift[(int64_t)b * a.rows + row] = (uint32_t)fminf(d, kMost) * (0x10001u << kBits);
+    }
+  }
+  if (strip) return;
   // the sums are of exponentials times 2^kExpBits
   sum *= __builtin_amdgcn_exp2f(-Elem<T>::kExpBits);
   constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
   const int g = a.row0 + row, y = a.lab[g];
-  float loss = __builtin_nanf("");
-  if (y >= 0) {
-    const float d = __builtin_fmaf(a.zy[g], kLog2e, -to);
-    loss = kLn2 * (log2f(sum) - d);
-    loss = loss < 0.0f ? 0.0f : loss;  // rounding; a NaN stays one
+  RowStat st = {top, __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+  if (y >= 0 && !(a.zy[g] > 3.4e38f)) {  // (a logit of +inf: NaN, as its exponential is no number)
+    const float d = __builtin_fmaf(a.zy[g], kLog2e, -top);  // label's power of two over the rest's
+    const float q = sum * __builtin_amdgcn_exp2f(-d);
+    st.loss = d < -60.0f ? kLn2 * (log2f(sum) - d) : log1pf(q);
+    st.miss = q > 1e30f ? 1.0f : q / (1.0f + q);
+    st.inv = 1.0f / (sum + __builtin_amdgcn_exp2f(d));
   }
-  RowStat st;
-  st.top = to;
-  st.inv = 1.0f / sum;
-  st.miss = -expm1f(-loss);
-  st.loss = loss;
   a.row[g] = st;
-  if (a.per_row && a.loss) a.loss[a.idx[g]] = loss;
+  if (a.per_row && a.loss) a.loss[a.idx[g]] = st.loss;
 }
 
 __global__ __launch_bounds__(1024) void k_ce_loss(CeArgs a) {
@@ -636,18 +664,23 @@ __global__ __launch_bounds__(256) void k_ce_dz(CeArgs a) {
 
 // ---- dh ---------------------------------------------------------------------------------------
 
-// part[z] [rows, D] = dz W over the z-th share of the vocabulary.
-template <typename T, int BM, int BN, int WM, int NS_>
+// part[z] [rows, D] = dz W over the z-th share of the vocabulary.  SHIFT: of the exponentials as
+// the logits product left them, relative to a power of two per row and block of columns, without
+// the label's: a fragment is brought to its row's power of two by subtracting binades from the
+// exponents, which is exact, and k_ce_dh_sum does the rest (1 / sum, the label's row of the table).
+// dz is then never written: at 1024 tokens of a vocabulary of 151936 k_ce_dz takes 92 us.
+template <typename T, int BM, int BN, int WM, int NS_, bool SHIFT>
 struct HiddenGrad {
   static constexpr int WN = kWaves / WM, NS = NS_, TM = BM / 32 / WM, TN = BN / 32 / WN;
   using B = ColTile<BN>;
-  static constexpr int A_BYTES = BM * kK * 2, NA = BM / 64;
-  static constexpr int STAGE = A_BYTES + B::BYTES, NCP = NA + B::N;
+  static constexpr int A_BYTES = BM * kK * 2, NA = BM / 64, S_BYTES = SHIFT ? 1024 : 0;
+  static constexpr int STAGE = A_BYTES + B::BYTES + S_BYTES, NCP = NA + B::N;
   const CeArgs& a;
   B cb;
   const char* ebase;
   int wave, lane, m0, n0, k0, wm0, wn0;
   int at[TN];
+  uint32_t now[TM], then[TM];
 
   __device__ __forceinline__ HiddenGrad(const CeArgs& args) : a(args) {
     wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -666,6 +699,10 @@ struct HiddenGrad {
       const int blk = wave * NA + c;
       copy1k(lds + blk * 1024,
              ebase + (int64_t)(k0 + k) * (a.rows / 32) * 4096 + blk * 1024, lane * 16);
+      // one wave's copy more than NCP: the counted waits then wait for more, not for less
+      if (SHIFT && c == 0 && wave == 0)
+        copy1k(lds + A_BYTES + B::BYTES,
+               a.shift + (int64_t)((k0 + k) * kK / a.stat_cols) * a.rows + m0, lane * 16);
     } else {
       cb.copy(lds + A_BYTES, k0 + k, a.V - 1, c - NA, wave);
     }
@@ -676,10 +713,34 @@ struct HiddenGrad {
   __device__ __forceinline__ u32x4 second(const char* s, int kk, int i) const {
     return *reinterpret_cast<const u32x4*>(s + (wm0 / 32 + i) * 4096 + kk * 1024 + lane * 16);
   }
-  __device__ __forceinline__ void fix(u32x4&, int) const {}
-  __device__ __forceinline__ void step(int, int) const {}
+  __device__ __forceinline__ void load(const char* s) {
+    if constexpr (SHIFT) {
+#pragma unroll
+      for (int i = 0; i < TM; i++)
+        then[i] = *reinterpret_cast<const uint32_t*>(
+            s + A_BYTES + B::BYTES + (wm0 + 32 * i + (lane & 31)) * 4);
+    }
+  }
+  __device__ __forceinline__ void next() {
+    if constexpr (SHIFT) {
+#pragma unroll
+      for (int i = 0; i < TM; i++) now[i] = then[i];
+    }
+  }
+  __device__ __forceinline__ void fix(u32x4& f, int i) const {
+    if constexpr (SHIFT) {
+      typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+      const ushort2_t n = __builtin_bit_cast(ushort2_t, now[i]);
+#pragma unroll
+      for (int q = 0; q < 4; q++) {  // below the smallest normal number: zero
+        const uint32_t x = f[q];  // (a bit cast of a vector's element would take the first one)
+        f[q] = __builtin_bit_cast(
+            uint32_t, __builtin_elementwise_sub_sat(__builtin_bit_cast(ushort2_t, x), n));
+      }
+    }
+  }
   __device__ __forceinline__ void done(int, float16_t (&acc)[TM][TN]) const {
-    float* out = a.part + (int64_t)blockIdx.z * a.rows * a.D;
+    float* out = a.part + (int64_t)(k0 / a.split_steps) * a.rows * a.D;
 #pragma unroll
     for (int i = 0; i < TM; i++) {
       float* row = out + (int64_t)(m0 + wm0 + 32 * i + (lane & 31)) * a.D;
@@ -697,20 +758,23 @@ struct HiddenGrad {
   }
 };
 
-template <typename T, int BM, int BN, int WM, int NS>
-__global__ __launch_bounds__(kThreads) void k_ce_dh(CeArgs a) {
+// Consecutive places are the column tiles of a row tile, then the row tiles of a share: an XCD's
+// 32 workgroups read few shares' operands (1024 tokens: one share, all of its tiles).
+template <typename T, int BM, int BN, int WM, int NS, bool SHIFT>
+__global__ __launch_bounds__(kThreads) void k_ce_dh(CeArgs a, int nx, int ny) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  using P = HiddenGrad<T, BM, BN, WM, NS>;
+  using P = HiddenGrad<T, BM, BN, WM, NS, SHIFT>;
   P p(a);
-  p.m0 = (int)blockIdx.y * BM;
-  p.n0 = (int)blockIdx.x * BN;
-  p.k0 = (int)blockIdx.z * a.split_steps;
+  const int at = xcd_place((int)blockIdx.x, (int)gridDim.x), x = at % nx, yz = at / nx;
+  p.m0 = yz % ny * BM;
+  p.n0 = x * BN;
+  p.k0 = yz / ny * a.split_steps;
   const int steps = min((a.V + kK - 1) / kK - p.k0, a.split_steps);
   if (p.m0 < piece_rows(a)) stream_tiles<T, P::TM, P::TN>(p, smem, 1, steps);
 }
 
 // dh rows = the shares' sum, with the scales, to their places in [T, D].
-template <typename T>
+template <typename T, bool SHIFT>
 __global__ __launch_bounds__(256) void k_ce_dh_sum(CeArgs a) {
   const int n = piece_rows(a), row = (int)blockIdx.y;
   const int d = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 4;
@@ -719,12 +783,25 @@ __global__ __launch_bounds__(256) void k_ce_dh_sum(CeArgs a) {
   const float* p = a.part + (int64_t)row * a.D + d;
   for (int z = 0; z < a.splits; z++)
     x += *reinterpret_cast<const float4_t*>(p + (int64_t)z * a.rows * a.D);
+  const int g = a.row0 + row, i = a.idx[g];
   float f = __builtin_amdgcn_exp2f(-Elem<T>::kGradBits);
-  if (a.row_grad) f *= a.gmax[0];
+  if constexpr (SHIFT) {
+    const RowStat st = a.row[g];
+    const int y = max(a.lab[g], 0);  // (a label outside the vocabulary: st is NaN)
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    const vec4 w = *reinterpret_cast<const vec4*>(static_cast<const T*>(a.w) +
+                                                  (int64_t)y * a.ldw + d);
+    const float inv = st.inv * __builtin_amdgcn_exp2f(-Elem<T>::kExpBits);
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] = x[e] * inv - st.miss * (float)w[e];
+    f = a.row_grad ? a.row_grad[i] : 1.0f;
+  } else {
+    if (a.row_grad) f *= a.gmax[0];
+  }
   if (a.mean) f /= (float)a.count[0];
 #pragma unroll
   for (int e = 0; e < 4; e++) x[e] *= f;
-  *reinterpret_cast<float4_t*>(a.dh + (int64_t)a.idx[a.row0 + row] * a.D + d) = x;
+  *reinterpret_cast<float4_t*>(a.dh + (int64_t)i * a.D + d) = x;
 }
 
 // ---- dW ---------------------------------------------------------------------------------------
@@ -761,7 +838,9 @@ struct TableGrad {
         eat[odd][x] = c * 1024 + b * 512 + (t ^ (4 * b + 8 * c)) * 16 + (s >> 1) * 8;
       }
   }
-  __device__ __forceinline__ int place(int q) const { return q * (int)gridDim.x + (int)blockIdx.x; }
+  __device__ __forceinline__ int place(int q) const {
+    return q * (int)gridDim.x + xcd_place((int)blockIdx.x, (int)gridDim.x);
+  }
   __device__ __forceinline__ void coords(int q, int& v, int& n) const {
     const int at = place(q);
     v = at / nt;
@@ -796,7 +875,8 @@ struct TableGrad {
     return (u32x4){x[0], x[1], y[0], y[1]};
   }
   __device__ __forceinline__ void fix(u32x4&, int) const {}
-  __device__ __forceinline__ void step(int, int) const {}
+  __device__ __forceinline__ void load(const char*) const {}
+  __device__ __forceinline__ void next() const {}
   __device__ __forceinline__ void done(int q, float16_t (&acc)[TM][TN]) const {
     int v, n;
     coords(q, v, n);
@@ -831,7 +911,7 @@ __global__ __launch_bounds__(kThreads) void k_ce_dw(CeArgs a) {
   P p(a);
   p.nt = (a.D + BN - 1) / BN;
   const int places = (a.V + P::BM - 1) / P::BM * p.nt, g = (int)gridDim.x;
-  const int wg = (int)blockIdx.x, tiles = wg < places ? (places - wg + g - 1) / g : 0;
+  const int wg = p.place(0), tiles = wg < places ? (places - wg + g - 1) / g : 0;
   const int steps = (piece_rows(a) + kK - 1) / kK;
   if (tiles == 0) return;
   if (steps > 0) {
@@ -917,7 +997,7 @@ static CePlan ce_plan(int T, int V, int D, bool grads, int cus) {
     while (most < p.Tp && most < 8192) most *= 2;  // 8 KB of statistics a row at 128 K columns
   p.pieces = (int)((p.Tp + most - 1) / most);
   p.rows = (int)((p.Tp / kRowPad + p.pieces - 1) / p.pieces) * kRowPad;
-  p.bm = T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
+  p.bm = T <= 32 && !grads ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
   p.stat_cols = p.bm == 256 ? 128 : p.bm == 32 ? 32 : 64;
   p.blocks = (int)(p.vp / p.stat_cols);
   p.dh_bm = T <= 64 ? 64 : 256;
@@ -944,7 +1024,7 @@ static CePlan ce_plan(int T, int V, int D, bool grads, int cus) {
 }
 
 struct CeLayout {
-  int64_t idx, lab, hc, row, zy, stat, e, part, end;
+  int64_t idx, lab, hc, row, zy, stat, shift, e, part, end;
 };
 
 static CeLayout ce_layout(const CePlan& p, int D, bool grads, bool dh) {
@@ -961,6 +1041,7 @@ static CeLayout ce_layout(const CePlan& p, int D, bool grads, bool dh) {
   l.row = take(16LL * p.Tp);
   l.zy = take(4LL * p.Tp);
   l.stat = take(8LL * p.blocks * p.rows);
+  l.shift = grads ? take(4LL * p.blocks * p.rows) : 0;
   l.e = grads ? take(2LL * p.vp * p.rows) : 0;
   l.part = dh ? take(4LL * p.splits * p.rows * D) : 0;
   l.end = at;
@@ -979,16 +1060,17 @@ static int launch_logits(const CeArgs& a, int cus, hipStream_t stream) {
   return ce_launched();
 }
 
-template <typename T, int BM, int BN, int WM, int NS>
+template <typename T, int BM, int BN, int WM, int NS, bool SHIFT>
 static int launch_dh(const CeArgs& a, const CePlan& p, hipStream_t stream) {
-  using P = HiddenGrad<T, BM, BN, WM, NS>;
+  using P = HiddenGrad<T, BM, BN, WM, NS, SHIFT>;
   static bool set[16];
-  auto* fn = &k_ce_dh<T, BM, BN, WM, NS>;
+  auto* fn = &k_ce_dh<T, BM, BN, WM, NS, SHIFT>;
   const int rc = ce_lds(fn, NS * P::STAGE, set);
   if (rc != MXS_OK) return rc;
   const int rows = a.rows < a.T ? a.rows : a.T;
-  hipLaunchKernelGGL(fn, dim3((a.D + BN - 1) / BN, (rows + BM - 1) / BM, p.splits),
-                     dim3(kThreads), NS * P::STAGE, stream, a);
+  const int nx = (a.D + BN - 1) / BN, ny = (rows + BM - 1) / BM;
+  hipLaunchKernelGGL(fn, dim3(nx * ny * p.splits), dim3(kThreads), NS * P::STAGE, stream, a, nx,
+                     ny);
   return ce_launched();
 }
 
@@ -1019,18 +1101,15 @@ static int logits_of(const CeArgs& a, const CePlan& p, int cus, hipStream_t stre
   }
 }
 
-template <typename T>
+template <typename T, bool SHIFT>
 static int dh_of(const CeArgs& a, const CePlan& p, hipStream_t stream) {
-  if (p.dh_bm == 64) {
-    switch (p.dh_bn) {
-      case 256: return launch_dh<T, 64, 256, 2, 3>(a, p, stream);
-      default: return launch_dh<T, 64, 128, 2, 3>(a, p, stream);
-    }
-  }
+  if (p.dh_bm == 64)
+    return p.dh_bn == 256 ? launch_dh<T, 64, 256, 2, 3, SHIFT>(a, p, stream)
+                          : launch_dh<T, 64, 128, 2, 3, SHIFT>(a, p, stream);
   switch (p.dh_bn) {
-    case 256: return launch_dh<T, 256, 256, 4, 2>(a, p, stream);
-    case 192: return launch_dh<T, 256, 192, 4, 2>(a, p, stream);
-    default: return launch_dh<T, 256, 128, 4, 3>(a, p, stream);
+    case 256: return launch_dh<T, 256, 256, 4, 2, SHIFT>(a, p, stream);
+    case 192: return launch_dh<T, 256, 192, 4, 2, SHIFT>(a, p, stream);
+    default: return launch_dh<T, 256, 128, 4, 3, SHIFT>(a, p, stream);
   }
 }
 
@@ -1040,29 +1119,37 @@ static int run_ce(CeArgs a, const CePlan& p, int cus, hipStream_t stream) {
   const int vec = (uintptr_t)a.h % 16 == 0 && a.ldh % 8 == 0;
   hipLaunchKernelGGL(k_ce_rows, dim3(p.Tp / kGather), dim3(256), 0, stream, a, vec);
   CE_TRY(ce_launched());
-  if (grads && a.row_grad) {
+  if (a.dw && a.row_grad) {
     hipLaunchKernelGGL(k_ce_gmax, dim3(1), dim3(1024), 0, stream, a);
     CE_TRY(ce_launched());
   }
+  const bool shift = a.dh && !a.dw;
   for (int i = 0; i < p.pieces; i++) {
     a.row0 = i * p.rows;
     a.rows = p.rows < p.Tp - a.row0 ? p.rows : p.Tp - a.row0;
     a.first = i == 0;
     CE_TRY(grads ? (logits_of<T, true>(a, p, cus, stream))
                  : (logits_of<T, false>(a, p, cus, stream)));
-    hipLaunchKernelGGL(k_ce_join<T>, dim3(a.rows / 32), dim3(1024), 0, stream, a);
+    if (shift)
+      hipLaunchKernelGGL((k_ce_join<T, true>), dim3(a.rows / kJoinRows), dim3(1024), 0, stream, a);
+    else
+      hipLaunchKernelGGL((k_ce_join<T, false>), dim3(a.rows / kJoinRows), dim3(1024), 0, stream, a);
     CE_TRY(ce_launched());
-    if (!grads) continue;
-    const int tbs = a.rows / 32, ys = 4096 / tbs + 1;
-    hipLaunchKernelGGL(k_ce_dz<T>, dim3(tbs, ys), dim3(256), 0, stream, a);
-    CE_TRY(ce_launched());
+    if (a.dw) {
+      const int tbs = a.rows / 32, ys = 4096 / tbs + 1;
+      hipLaunchKernelGGL(k_ce_dz<T>, dim3(tbs, ys), dim3(256), 0, stream, a);
+      CE_TRY(ce_launched());
+      CE_TRY((launch_dw<T, 256, 2>(a, cus, stream)));
+    }
     if (a.dh) {
-      CE_TRY(dh_of<T>(a, p, stream));
-      hipLaunchKernelGGL(k_ce_dh_sum<T>, dim3((a.D / 4 + 255) / 256, a.rows), dim3(256), 0,
-                         stream, a);
+      CE_TRY(shift ? (dh_of<T, true>(a, p, stream)) : (dh_of<T, false>(a, p, stream)));
+      const dim3 grid((a.D / 4 + 255) / 256, a.rows);
+      if (shift)
+        hipLaunchKernelGGL((k_ce_dh_sum<T, true>), grid, dim3(256), 0, stream, a);
+      else
+        hipLaunchKernelGGL((k_ce_dh_sum<T, false>), grid, dim3(256), 0, stream, a);
       CE_TRY(ce_launched());
     }
-    if (a.dw) CE_TRY((launch_dw<T, 256, 2>(a, cus, stream)));
   }
   if (a.loss && !a.per_row) {
     hipLaunchKernelGGL(k_ce_loss, dim3(1), dim3(1024), 0, stream, a);
@@ -1122,6 +1209,7 @@ int mxs_head_ce(const void* h, int64_t ldh, const void* w, int64_t ldw, const in
   a.row = reinterpret_cast<RowStat*>(ws + l.row);
   a.zy = reinterpret_cast<float*>(ws + l.zy);
   a.stat = reinterpret_cast<float2*>(ws + l.stat);
+  a.shift = reinterpret_cast<uint32_t*>(ws + l.shift);
   a.e = reinterpret_cast<u32x4*>(ws + l.e);
   a.part = reinterpret_cast<float*>(ws + l.part);
   a.stat_cols = p.stat_cols;

@@ -5,6 +5,8 @@ Tolerances, u = 2^-24 and r half a step of the element type (fp16 2^-11, bf16 2^
 - a logit sums D products in fp32: e_z = D u max_v sum_d |h_d w_vd| per row;
 - a loss: e_z twice (the label's and the sum's), the exponentials' and the logarithm's own (4 u
   |z|), and sums of at most 128 terms in a chain (128 u): e_l = 2 e_z + u (4 max |z| + 128);
+- without the table's gradient fp16 exponentials keep 29 binades below a row's largest but the
+  label's, p'; each smaller one is off by at most 2^-29 p';
 - a weight p of dz is off by e_p = 2 e_l relative; dz is rounded twice on its way (2 r), and below
   fp16's normal range (times 2^14) by 2^-39; products sum in fp32 over n terms (n u), so a
   gradient is within (2 r + e_p + n u + 8 u) sum |dz| |other factor|, plus 2^-39 sum |other factor|,
@@ -60,10 +62,12 @@ def _exact(h, w, y, reduction, g, ignore=-100):
         dw += dz.t() @ x
         e_p = 2 * e_l[:, None]
         p = (z - lse[:, None]).exp() * per[some].abs()[:, None]  # what carries e_p
-        p[at, y[some]] += per[some].abs() * 0
         rel = 2 * r + (vocab + 8) * U
         small = 2.0 ** -39 * big
-        dh_tol[some] = rel * (dz.abs() @ w64.abs()) + e_p * (p @ w64.abs()) + \
+        other = p.clone()
+        other[at, y[some]] = 0
+        cut = 2.0 ** -29 * other.amax(1, keepdim=True) if h.dtype == F16 else 0.0
+        dh_tol[some] = cut * w64.abs().sum(0) + rel * (dz.abs() @ w64.abs()) + e_p * (p @ w64.abs()) + \
             small * w64.abs().sum(0)
         rel = 2 * r + (len(rows) + 8) * U
         dw_tol += rel * (dz.abs().t() @ x.abs()) + (e_p * p).t() @ x.abs() + \
