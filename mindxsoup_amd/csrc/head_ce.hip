@@ -21,7 +21,7 @@ namespace mxs {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kK = 64;             // reduction step: four MFMAs of 16
+constexpr int kK = 32;             // reduction step: two MFMAs of 16
 constexpr int kWaves = 8;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kRowPad = 256;       // gathered rows are padded with zeros to a multiple of this
@@ -91,7 +91,7 @@ struct CeArgs {
   float* zy;         // [Tp] the label's logit
   float2* stat;      // [blocks][piece rows] power of two and sum of a block of columns
   uint32_t* shift;   // [blocks][piece rows] binades from a block's to its row's power of two
-  u32x4* e;          // [Vp / 64][piece rows / 32][4][64] fragments of exponentials, then dz
+  u32x4* e;          // [Vp / 32][piece rows / 32][2][64] fragments of exponentials, then dz
   float* part;       // [splits][piece rows][D]
   // the piece
   int row0, rows;    // first gathered row, rows (a multiple of kRowPad)
@@ -221,34 +221,45 @@ __device__ __forceinline__ u32x2 read_tr(const char* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)p));
 }
 
-// An operand [ROWS][kK] whose reduction index is contiguous.  128-byte LDS rows of eight 16-byte
-// segments, segment s of row r at s ^ (r / 2 % 8): the 32 rows of a fragment read then fall on
-// all banks alike.  A fragment: row lane % 32, reduction indexes 8 (lane / 32) .. + 7.
+// Copies of one operand's stage: pieces of 1 KB, piece wave + 8 i copy i of a wave.  Where they do
+// not share out evenly, the waves behind the last piece have one copy less.
+template <int BYTES>
+struct Share {
+  static constexpr int PIECES = BYTES / 1024, N = (PIECES + kWaves - 1) / kWaves;
+  static constexpr bool kEven = PIECES % kWaves == 0;
+  __device__ __forceinline__ static bool mine(int i, int wave) {
+    return kEven || i + 1 < N || wave + kWaves * i < PIECES;
+  }
+};
+
+// An operand [ROWS][kK] whose reduction index is contiguous.  64-byte LDS rows of four 16-byte
+// segments, segment s of row r at s ^ (r / 4 % 4): 16 rows of a fragment read then fall on all
+// banks.  A fragment: row lane % 32, reduction indexes 8 (lane / 32) .. + 7 of its 16.
 template <int ROWS>
-struct RowTile {
-  static constexpr int BYTES = ROWS * kK * 2, N = (ROWS + 63) / 64;
+struct RowTile : Share<ROWS * kK * 2> {
+  static constexpr int BYTES = ROWS * kK * 2;
+  using Share<BYTES>::N;
   uint32_t off[N];
   const char* base;
-  int read0;  // byte offset of the lane's row and (first) segment
 
   // rows row0 .. of src, those past `last` repeating it
   __device__ __forceinline__ void tile(const void* src, int64_t ld, int row0, int last, int wave,
                                        int lane) {
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const int row = (wave * 8 + 64 * i + (lane >> 3)) % ROWS;
-      const int seg = ((lane & 7) ^ (row >> 1)) & 7;
+      const int row = (wave + kWaves * i) * 16 + (lane >> 2);
+      const int seg = (lane & 3) ^ ((row >> 2) & 3);
       off[i] = ((uint32_t)min(row, last - row0) * (uint32_t)ld + seg * 8) * 2;
     }
     base = static_cast<const char*>(src) + (int64_t)row0 * ld * 2;
   }
   __device__ __forceinline__ void copy(uint32_t lds, int k, int i, int wave) const {
-    copy1k(lds + (wave * 8 + 64 * i) % ROWS * 128, base + (int64_t)k * (kK * 2), off[i]);
+    copy1k(lds + (wave + kWaves * i) * 1024, base + (int64_t)k * (kK * 2), off[i]);
   }
   __device__ __forceinline__ static u32x4 read(const char* s, int row0, int kk, int lane) {
     const int row = row0 + (lane & 31);
-    const int seg = (2 * kk + (lane >> 5)) ^ ((row >> 1) & 7);
-    return *reinterpret_cast<const u32x4*>(s + row * 128 + seg * 16);
+    const int seg = (2 * kk + (lane >> 5)) ^ ((row >> 2) & 3);
+    return *reinterpret_cast<const u32x4*>(s + row * 64 + seg * 16);
   }
 };
 
@@ -257,9 +268,10 @@ struct RowTile {
 // row length already puts odd rows on the other half of the banks).  A fragment: column
 // lane % 32, reduction indexes 4 h .. + 3 and 8 + 4 h .. + 3 of its 16 (h = lane / 32).
 template <int COLS>
-struct ColTile {
-  static constexpr int BYTES = COLS * kK * 2, N = COLS / 64, SEGS = COLS / 8;
-  static constexpr bool kHalf = COLS % 128 != 0;  // 64-column multiples: rows 32 dwords apart
+struct ColTile : Share<COLS * kK * 2> {
+  static constexpr int BYTES = COLS * kK * 2, SEGS = COLS / 8;
+  using Share<BYTES>::N;
+  static constexpr bool kHalf = COLS % 128 != 0;  // rows 32 banks apart
   int row_[N], seg8[N];
   const char* base;
   int64_t ld2;
@@ -306,22 +318,31 @@ struct ColTile {
 // vocabulary: no transposition anywhere.
 
 // Runs a workgroup's `tiles` tiles of `steps` reduction steps.  P: the operands.
-//   enter(q)           copies from now on are of tile q
-//   copy(stage, k, c)  copy c of P::NCP of reduction step k
+//   enter(q)              copies from now on are of tile q
+//   copy(lds, q, k, c)    copy c of P::NCP of step k of tile q into the stage at LDS address lds
+//   lean                  this wave has P::NCP - 1 copies a step
 //   first(s, kk, j), second(s, kk, i): fragments of sub-step kk of the stage at s
-//   fix(f, i)          applied to second's fragment before its products
-//   load(s), next()    what fix needs of the reduction step in stage s: read, then taken over
-//   done(q, acc)       tile q's sums; acc[i][j] = first_j x second_i
-// Sub-step order, copies and barriers: a step's last sub-step is multiplied behind the barrier
-// that ends it, over the next step's first reads; the stage that this barrier frees takes the
-// copies of the step after P::NS, spread over that sub-step and the next two.
+//   fix(f, i)             applied to second's fragment before its products
+//   load(s), next()       what fix needs of the step in the stage at s: read, then taken over
+//   done(q, acc)          tile q's sums; acc[i][j] = first_j x second_i; whether this wave issued
+//                         P::STORES stores or more
+// P::NS stages of one 32-deep step each, so that P::NS - 1 steps' copies are under way: with two
+// stages of 64 the copies had less than a step to land, and a step of dh at 256 x 192 took 1.6 us
+// instead of the 0.64 of its products.  A step's second half is multiplied behind the barrier that
+// ends it, over the next step's first reads; the stage that this barrier frees takes the copies
+// of the step after P::NS, over that half and the next step's first one.
+// Waits count what was issued after the copies they wait for (vmcnt retires in order): the copies
+// of P::NS - 2 steps, and behind a tile's end, while those copies were issued before it, its
+// stores, which so have some steps' time to drain.
 template <typename T, int TM, int TN, typename P>
 __device__ __forceinline__ void stream_tiles(P& p, char* smem, int tiles, int steps) {
-  constexpr int NS = P::NS, NCP = P::NCP, NRD = TM + TN, NMF = TM * TN;
+  constexpr int NS = P::NS, NCP = P::NCP, NRD = TM + TN, NMF = TM * TN, HALF = (NCP + 1) / 2;
+  static_assert((NS - 2) * NCP + P::STORES <= 63, "vmcnt is 6 bits");
   float16_t acc[TM][TN];
   u32x4 f1[2][TN], f2[2][TM];
   int ct = 0, ck = 0, cstage = 0;  // the copies' tile, step and stage
   const uint32_t lds0 = lds_addr(smem);
+  auto copy = [&](int c) { p.copy(lds0 + cstage * P::STAGE, ct, ck, c); };
   auto advance = [&]() {  // to the next step; the last one is copied again rather than none
     cstage = cstage + 1 == NS ? 0 : cstage + 1;
     if (ck + 1 < steps) ck++;
@@ -335,10 +356,10 @@ __device__ __forceinline__ void stream_tiles(P& p, char* smem, int tiles, int st
 #pragma unroll
   for (int s = 0; s < NS; s++) {
 #pragma unroll
-    for (int c = 0; c < (s + 1 < NS ? NCP : NCP / 3); c++) p.copy(lds0 + cstage * P::STAGE, ck, c);
+    for (int c = 0; c < (s + 1 < NS ? NCP : HALF); c++) copy(c);
     if (s + 1 < NS) advance();
   }
-  wait_vmcnt<(NS - 2) * NCP + NCP / 3>();
+  wait_vmem_all();
   lds_barrier();
   auto read = [&](int set, const char* s, int kk, int e) {
     if (e == 0 || e > TN) {
@@ -352,10 +373,8 @@ __device__ __forceinline__ void stream_tiles(P& p, char* smem, int tiles, int st
   for (int e = 0; e < NRD; e++) read(0, smem, 0, e);
   p.load(smem);
   p.next();
-  // multiply set `set`; read sub-step kk of the stage at s into the other one; third `part` of the
-  // copies of the copies' step
-  auto sub = [&](int set, const char* s, int kk, int part) {
-    const int c0 = part < 0 ? 0 : part * NCP / 3, c1 = part < 0 ? 0 : (part + 1) * NCP / 3;
+  // multiply set `set`; read sub-step kk of the stage at s into the other one; copies c0 .. c1 - 1
+  auto sub = [&](int set, const char* s, int kk, int c0, int c1) {
     int c = c0;
 #pragma unroll
     for (int i = 0; i < TM; i++) p.fix(f2[set][i], i);
@@ -366,12 +385,11 @@ __device__ __forceinline__ void stream_tiles(P& p, char* smem, int tiles, int st
 #pragma unroll
       for (int q = e * NRD / NMF; q < (e + 1) * NRD / NMF; q++) read(set ^ 1, s, kk, q);
 #pragma unroll
-      for (; c < c1 && (e + 1) * (c1 - c0) >= (c - c0 + 1) * NMF; c++)
-        p.copy(lds0 + cstage * P::STAGE, ck, c);
+      for (; c < c1 && (e + 1) * (c1 - c0) >= (c - c0 + 1) * NMF; c++) copy(c);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  int stage = 0;
+  int stage = 0, stored = 0;  // steps whose wait may leave the last tile's stores
   for (int q = 0; q < tiles; q++) {
 #pragma unroll
     for (int i = 0; i < TM; i++)
@@ -380,19 +398,23 @@ __device__ __forceinline__ void stream_tiles(P& p, char* smem, int tiles, int st
 #pragma unroll
         for (int r = 0; r < 16; r++) acc[i][j][r] = 0.0f;
     for (int k = 0; k < steps; k++) {
-      const char* s = smem + stage * P::STAGE;
-      sub(0, s, 1, 1);
-      sub(1, s, 2, 2);
+      sub(0, smem + stage * P::STAGE, 1, HALF, NCP);
       advance();
-      sub(0, s, 3, -1);
-      wait_vmcnt<(NS - 2) * NCP>();
+      if (stored > 0) {
+        stored--;
+        if (p.lean) wait_vmcnt<(NS - 2) * (NCP - 1) + P::STORES>();
+        else wait_vmcnt<(NS - 2) * NCP + P::STORES>();
+      } else {
+        if (p.lean) wait_vmcnt<(NS - 2) * (NCP - 1)>();
+        else wait_vmcnt<(NS - 2) * NCP>();
+      }
       lds_barrier();
       stage = stage + 1 == NS ? 0 : stage + 1;
       p.load(smem + stage * P::STAGE);
-      sub(1, smem + stage * P::STAGE, 0, 0);
+      sub(1, smem + stage * P::STAGE, 0, 0, HALF);
       p.next();
     }
-    p.done(q, acc);
+    stored = p.done(q, acc) ? NS - 2 : 0;
   }
   wait_vmem_all();  // no copy may land after the workgroup's end
 }
@@ -415,14 +437,22 @@ struct Logits {
   using A = RowTile<BM>;
   using B = RowTile<BN>;
   static constexpr int STAGE = A::BYTES + B::BYTES, NCP = A::N + B::N;
+  // Labels of a tile's rows, copied with its first step: a load in the epilogue would wait for
+  // every copy before it.  The copies are at most three tiles ahead (two steps a tile at least).
+  static constexpr int SLOTS = 4, LDS = NS * STAGE + SLOTS * 1024;
+  static_assert((NS + 1) / 2 < SLOTS && A::kEven + B::kEven > 0, "label slots, copies per wave");
+  static constexpr int STORES = KEEP ? TM * TN * 2 : 0;  // at least: 16 bytes a lane is the widest
   const CeArgs& a;
+  const char* smem;
   A ca;
   B cb;
-  int wave, lane, rows, mt, seq0, seqs, wm0, wn0;
+  int wave, lane, mt, wm0, wn0, m_copy;
+  bool lean;
 
-  __device__ __forceinline__ Logits(const CeArgs& args) : a(args) {
+  __device__ __forceinline__ Logits(const CeArgs& args, const char* lds) : a(args), smem(lds) {
     wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     lane = threadIdx.x & 63;
+    lean = !(A::mine(A::N - 1, wave) && B::mine(B::N - 1, wave));
     wm0 = wave / WN * (BM / WM);
     wn0 = wave % WN * COLS;
   }
@@ -438,15 +468,22 @@ struct Logits {
     m = rest >> 2;
   }
   __device__ __forceinline__ void enter(int q) {
-    int vt, m;
-    coords(place(q), vt, m);
+    int vt;
+    coords(place(q), vt, m_copy);
     const int last = a.V - 1, v0 = min(vt * BN, last);
-    ca.tile(a.hc, a.D, a.row0 + m * BM, a.row0 + a.rows - 1, wave, lane);
+    ca.tile(a.hc, a.D, a.row0 + m_copy * BM, a.row0 + a.rows - 1, wave, lane);
     cb.tile(a.w, a.ldw, v0, last, wave, lane);
   }
-  __device__ __forceinline__ void copy(uint32_t lds, int k, int c) const {
-    if (c < A::N) ca.copy(lds, k, c, wave);
-    else cb.copy(lds + A::BYTES, k, c - A::N, wave);
+  __device__ __forceinline__ void copy(uint32_t lds, int q, int k, int c) const {
+    // one wave's copy more than NCP: the counted waits then wait for more, not for less
+    if (c == 0 && k == 0 && wave == 0)
+      copy1k(lds_addr(smem) + NS * STAGE + q % SLOTS * 1024, a.lab + a.row0 + m_copy * BM,
+             lane * 16);
+    if (c < A::N) {
+      if (A::mine(c, wave)) ca.copy(lds, k, c, wave);
+    } else {
+      if (B::mine(c - A::N, wave)) cb.copy(lds + A::BYTES, k, c - A::N, wave);
+    }
   }
   __device__ __forceinline__ u32x4 first(const char* s, int kk, int j) const {
     return B::read(s + A::BYTES, wn0 + 32 * j, kk, lane);
@@ -459,11 +496,11 @@ struct Logits {
   __device__ __forceinline__ void next() const {}
 
   // acc[i][j][r]: row 32 i + lane % 32, column 32 j + 8 (r / 4) + 4 (lane / 32) + r % 4.
-  __device__ __forceinline__ void done(int q, float16_t (&acc)[TM][TN]) const {
+  __device__ __forceinline__ bool done(int q, float16_t (&acc)[TM][TN]) const {
     int vt, m;
     coords(place(q), vt, m);
     const int v0 = vt * BN + wn0;
-    if (vt * BN >= a.V) return;
+    if (vt * BN >= a.V) return false;
     const int h = lane >> 5;
     if (v0 + COLS > a.V) {  // columns past the vocabulary
 #pragma unroll
@@ -480,7 +517,8 @@ struct Logits {
 #pragma unroll
     for (int i = 0; i < TM; i++) {
       const int row = m * BM + wm0 + 32 * i + (lane & 31);  // of the piece
-      const int y = a.lab[a.row0 + row] - v0;  // the label's column of this wave
+      const int y = reinterpret_cast<const int*>(  // the label's column of this wave
+                        smem + NS * STAGE + q % SLOTS * 1024)[wm0 + 32 * i + (lane & 31)] - v0;
       if (__any(y >= 0 && y < COLS)) {  // the label's logit goes to zy alone
 #pragma unroll
         for (int j = 0; j < TN; j++)
@@ -503,7 +541,7 @@ struct Logits {
       float sum = 0.0f;
       u32x4* e = nullptr;
       if constexpr (KEEP)
-        e = a.e + ((int64_t)(v0 / kK) * (a.rows / 32) + (row >> 5)) * 256 + lane;
+        e = a.e + ((int64_t)(v0 / kK) * (a.rows / 32) + (row >> 5)) * 128 + lane;
 #pragma unroll
       for (int j = 0; j < TN; j++) {
         u32x4 f[2];
@@ -516,8 +554,7 @@ struct Logits {
           if constexpr (KEEP) f[r >> 3][(r & 7) >> 1] = Elem<T>::pack(x, z);
         }
         if constexpr (KEEP) {
-          u32x4* to = e + (int64_t)((v0 % kK + 32 * j) / kK) * (a.rows / 32) * 256 +
-                      (v0 % kK + 32 * j) % kK / 16 * 64;
+          u32x4* to = e + (int64_t)j * (a.rows / 32) * 128;
           to[0] = f[0];
           to[64] = f[1];
         }
@@ -525,6 +562,7 @@ struct Logits {
       sum += __shfl_xor(sum, 32);
       if (h == 0) a.stat[(int64_t)(v0 / COLS) * a.rows + row] = make_float2(top, sum);
     }
+    return KEEP;
   }
 };
 
@@ -532,7 +570,7 @@ template <typename T, int BM, int WM, int NS, bool KEEP>
 __global__ __launch_bounds__(kThreads) void k_ce_logits(CeArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using P = Logits<T, BM, WM, NS, KEEP>;
-  P p(a);
+  P p(a, smem);
   p.mt = (piece_rows(a) + BM - 1) / BM;
   const int vt = (a.V + P::BN - 1) / P::BN, places = (vt + 3) / 4 * 4 * p.mt;
   const int g = (int)gridDim.x, wg = p.place(0);
@@ -620,7 +658,7 @@ __global__ __launch_bounds__(1024) void k_ce_loss(CeArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void k_ce_dz(CeArgs a) {
   const int n = piece_rows(a), tbs = a.rows / 32, live = (n + 255) / 256 * 8;
-  const int lane = threadIdx.x & 63, kk = threadIdx.x >> 6, tb = (int)blockIdx.x;
+  const int lane = threadIdx.x & 63, b = threadIdx.x >> 6, tb = (int)blockIdx.x;
   if (tb >= live) return;
   const int row = tb * 32 + (lane & 31), h = lane >> 5, g = a.row0 + row;
   float f = 0.0f, top = 0.0f, at_label = 0.0f;
@@ -636,10 +674,10 @@ __global__ __launch_bounds__(256) void k_ce_dz(CeArgs a) {
     at_label = -st.miss * scale;
     top = st.top;
   }
-  const int steps = (a.V + kVocabTile - 1) / kVocabTile * (kVocabTile / kK);
-  for (int s = (int)blockIdx.y; s < steps; s += (int)gridDim.y) {
-    const int v0 = s * kK + kk * 16;
-    u32x4* p = a.e + ((int64_t)s * tbs + tb) * 256 + threadIdx.x;
+  const int pairs = (a.V + kVocabTile - 1) / kVocabTile * (kVocabTile / 64);
+  for (int s = (int)blockIdx.y; s < pairs; s += (int)gridDim.y) {
+    const int v0 = s * 64 + b * 16;
+    u32x4* p = a.e + ((int64_t)(v0 / kK) * tbs + tb) * 128 + (b & 1) * 64 + lane;
     u32x4 x = *p;
     float w = 0.0f;
     if (row < n && v0 < a.V)
@@ -673,18 +711,23 @@ template <typename T, int BM, int BN, int WM, int NS_, bool SHIFT>
 struct HiddenGrad {
   static constexpr int WN = kWaves / WM, NS = NS_, TM = BM / 32 / WM, TN = BN / 32 / WN;
   using B = ColTile<BN>;
-  static constexpr int A_BYTES = BM * kK * 2, NA = BM / 64, S_BYTES = SHIFT ? 1024 : 0;
-  static constexpr int STAGE = A_BYTES + B::BYTES + S_BYTES, NCP = NA + B::N;
+  static constexpr int A_BYTES = BM * kK * 2, S_BYTES = SHIFT ? 1024 : 0;
+  using A = Share<A_BYTES>;
+  static constexpr int STAGE = A_BYTES + B::BYTES + S_BYTES, NCP = A::N + B::N, STORES = 0;
+  static constexpr int LDS = NS * STAGE;
+  static_assert(A::kEven + B::kEven > 0, "copies per wave");
   const CeArgs& a;
   B cb;
   const char* ebase;
   int wave, lane, m0, n0, k0, wm0, wn0;
+  bool lean;
   int at[TN];
   uint32_t now[TM], then[TM];
 
   __device__ __forceinline__ HiddenGrad(const CeArgs& args) : a(args) {
     wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     lane = threadIdx.x & 63;
+    lean = !(A::mine(A::N - 1, wave) && B::mine(B::N - 1, wave));
     wm0 = wave / WN * (BM / WM);
     wn0 = wave % WN * (BN / WN);
 #pragma unroll
@@ -692,26 +735,27 @@ struct HiddenGrad {
   }
   __device__ __forceinline__ void enter(int) {
     cb.tile(a.w, a.ldw, n0, a.D, wave, lane);
-    ebase = reinterpret_cast<const char*>(a.e) + (int64_t)(m0 / 32) * 4096;
+    ebase = reinterpret_cast<const char*>(a.e) + (int64_t)(m0 / 32) * 2048;
   }
-  __device__ __forceinline__ void copy(uint32_t lds, int k, int c) const {
-    if (c < NA) {
-      const int blk = wave * NA + c;
-      copy1k(lds + blk * 1024,
-             ebase + (int64_t)(k0 + k) * (a.rows / 32) * 4096 + blk * 1024, lane * 16);
+  __device__ __forceinline__ void copy(uint32_t lds, int, int k, int c) const {
+    if (c < A::N) {
+      const int blk = wave + kWaves * c;
+      if (A::mine(c, wave))
+        copy1k(lds + blk * 1024,
+               ebase + (int64_t)(k0 + k) * (a.rows / 32) * 2048 + blk * 1024, lane * 16);
       // one wave's copy more than NCP: the counted waits then wait for more, not for less
       if (SHIFT && c == 0 && wave == 0)
         copy1k(lds + A_BYTES + B::BYTES,
                a.shift + (int64_t)((k0 + k) * kK / a.stat_cols) * a.rows + m0, lane * 16);
     } else {
-      cb.copy(lds + A_BYTES, k0 + k, a.V - 1, c - NA, wave);
+      if (B::mine(c - A::N, wave)) cb.copy(lds + A_BYTES, k0 + k, a.V - 1, c - A::N, wave);
     }
   }
   __device__ __forceinline__ u32x4 first(const char* s, int kk, int j) const {
     return B::read(s + A_BYTES, at[j], kk);
   }
   __device__ __forceinline__ u32x4 second(const char* s, int kk, int i) const {
-    return *reinterpret_cast<const u32x4*>(s + (wm0 / 32 + i) * 4096 + kk * 1024 + lane * 16);
+    return *reinterpret_cast<const u32x4*>(s + (wm0 / 32 + i) * 2048 + kk * 1024 + lane * 16);
   }
   __device__ __forceinline__ void load(const char* s) {
     if constexpr (SHIFT) {
@@ -739,7 +783,7 @@ struct HiddenGrad {
       }
     }
   }
-  __device__ __forceinline__ void done(int, float16_t (&acc)[TM][TN]) const {
+  __device__ __forceinline__ bool done(int, float16_t (&acc)[TM][TN]) const {
     float* out = a.part + (int64_t)(k0 / a.split_steps) * a.rows * a.D;
 #pragma unroll
     for (int i = 0; i < TM; i++) {
@@ -755,6 +799,7 @@ struct HiddenGrad {
                            acc[i][j][4 * g + 3]};
         }
     }
+    return false;
   }
 };
 
@@ -814,12 +859,16 @@ template <typename T, int BN, int NS_>
 struct TableGrad {
   static constexpr int BM = 256, WM = 4, WN = 2, NS = NS_, TM = 2, TN = BN / 64;
   using B = ColTile<BN>;
-  static constexpr int A_BYTES = BM * kK * 2, NA = 4;
-  static constexpr int STAGE = A_BYTES + B::BYTES, NCP = NA + B::N;
+  static constexpr int A_BYTES = BM * kK * 2;
+  using A = Share<A_BYTES>;
+  static constexpr int STAGE = A_BYTES + B::BYTES, NCP = A::N + B::N;
+  static constexpr int STORES = TM * TN * 4, LDS = NS * STAGE;
+  static_assert(A::kEven && B::kEven, "copies per wave");
+  static constexpr bool lean = false;
   const CeArgs& a;
   B cb;
   const char* ebase;
-  int wave, lane, nt, n0, wm0, wn0;
+  int wave, lane, nt, wm0, wn0;
   int at[TN], eat[2][2];
 
   __device__ __forceinline__ TableGrad(const CeArgs& args) : a(args) {
@@ -831,7 +880,7 @@ struct TableGrad {
     for (int j = 0; j < TN; j++) at[j] = B::read_at(wn0 + 32 * j, lane);
     const int r = (lane & 15) >> 2, s = lane & 3, c = (lane >> 4) & 1, b = s & 1;
 #pragma unroll
-    for (int odd = 0; odd < 2; odd++)  // sub-step's parity: rows 16 odd .. of a block
+    for (int odd = 0; odd < 2; odd++)  // sub-step: rows 16 odd .. of a block
 #pragma unroll
       for (int x = 0; x < 2; x++) {
         const int t = 16 * odd + 8 * x + 4 * (lane >> 5) + r;
@@ -851,33 +900,30 @@ struct TableGrad {
     coords(q, v, n);
     cb.tile(static_cast<const uint16_t*>(a.hc) + (int64_t)a.row0 * a.D, a.D, n * BN, a.D, wave,
             lane);
-    ebase = reinterpret_cast<const char*>(a.e) + (int64_t)v * 4 * (a.rows / 32) * 4096;
+    ebase = reinterpret_cast<const char*>(a.e) + (int64_t)v * (BM / kK) * (a.rows / 32) * 2048;
   }
-  __device__ __forceinline__ void copy(uint32_t lds, int k, int c) const {
-    if (c < NA) {  // wave: columns 64 (wave / 2) .., rows 32 (wave % 2) ..; c: 16 columns
-      const int swap = 4 * (lane >> 5) + 8 * (c & 1);
+  __device__ __forceinline__ void copy(uint32_t lds, int, int k, int c) const {
+    if (c < A::N) {  // block of 16 table rows; 32 rows of h
+      const int blk = wave + kWaves * c, swap = 4 * (lane >> 5) + 8 * (blk & 1);
       const uint32_t off = ((lane & 32) + ((lane & 31) ^ swap)) * 16;
-      copy1k(lds + wave * 4096 + c * 1024,
-             ebase + ((int64_t)(wave >> 1) * (a.rows / 32) + 2 * k + (wave & 1)) * 4096 +
-                 c * 1024,
-             off);
+      copy1k(lds + blk * 1024,
+             ebase + ((int64_t)(blk >> 1) * (a.rows / 32) + k) * 2048 + (blk & 1) * 1024, off);
     } else {
-      cb.copy(lds + A_BYTES, k, a.rows - 1, c - NA, wave);
+      cb.copy(lds + A_BYTES, k, a.rows - 1, c - A::N, wave);
     }
   }
   __device__ __forceinline__ u32x4 first(const char* s, int kk, int j) const {
     return B::read(s + A_BYTES, at[j], kk);
   }
   __device__ __forceinline__ u32x4 second(const char* s, int kk, int i) const {
-    const int block = wm0 / 32 + i;  // 32 table rows: half of a 64-column group
-    const char* p = s + (block >> 1) * 8192 + (kk >> 1) * 4096 + (block & 1) * 2048;
-    const u32x2 x = read_tr(p + eat[kk & 1][0]), y = read_tr(p + eat[kk & 1][1]);
+    const char* p = s + (wm0 / 32 + i) * 2048;
+    const u32x2 x = read_tr(p + eat[kk][0]), y = read_tr(p + eat[kk][1]);
     return (u32x4){x[0], x[1], y[0], y[1]};
   }
   __device__ __forceinline__ void fix(u32x4&, int) const {}
   __device__ __forceinline__ void load(const char*) const {}
   __device__ __forceinline__ void next() const {}
-  __device__ __forceinline__ void done(int q, float16_t (&acc)[TM][TN]) const {
+  __device__ __forceinline__ bool done(int q, float16_t (&acc)[TM][TN]) const {
     int v, n;
     coords(q, v, n);
     float f = __builtin_amdgcn_exp2f(-Elem<T>::kGradBits);
@@ -901,6 +947,7 @@ struct TableGrad {
           *reinterpret_cast<float4_t*>(out + d) = x;
         }
     }
+    return (v + 1) * BM <= a.V && (n + 1) * BN <= a.D;  // else some stores fall away
   }
 };
 
@@ -1007,11 +1054,11 @@ static CePlan ce_plan(int T, int V, int D, bool grads, int cus) {
   for (int bn : {256, 192, 128}) {
     if (bn == 192 && p.dh_bm == 64) continue;  // six column blocks do not share out over the waves
     const int tiles = mt * ((D + bn - 1) / bn);
-    for (int s = 1; s <= 64 && s <= (steps + 7) / 8; s++) {
+    for (int s = 1; s <= 64 && s <= (steps + 15) / 16; s++) {
       const int per = (steps + s - 1) / s, z = (steps + per - 1) / per;
       const int rounds = (tiles * z + cus - 1) / cus;
       // a step's cost by its tile's width, the shares' sums as traffic
-      const double cost = rounds * (per * (0.25 + bn / 256.0) + 12) + 0.25 * z * mt;
+      const double cost = rounds * (per * (0.25 + bn / 256.0) + 24) + 0.5 * z * mt;
       if (best == 0 || cost < best) {
         best = cost;
         p.dh_bn = bn;
@@ -1036,7 +1083,7 @@ static CeLayout ce_layout(const CePlan& p, int D, bool grads, bool dh) {
     return o;
   };
   l.idx = take(4LL * p.Tp);
-  l.lab = take(4LL * p.Tp);
+  l.lab = take(4LL * (p.Tp + 256));  // copied in whole KB
   l.hc = take(2LL * p.Tp * D);
   l.row = take(16LL * p.Tp);
   l.zy = take(4LL * p.Tp);
@@ -1053,10 +1100,10 @@ static int launch_logits(const CeArgs& a, int cus, hipStream_t stream) {
   using P = Logits<T, BM, WM, NS, KEEP>;
   static bool set[16];
   auto* fn = &k_ce_logits<T, BM, WM, NS, KEEP>;
-  const int rc = ce_lds(fn, NS * P::STAGE, set);
+  const int rc = ce_lds(fn, P::LDS, set);
   if (rc != MXS_OK) return rc;
-  const int per_cu = 2 * NS * P::STAGE <= 160 * 1024 ? 2 : 1;
-  hipLaunchKernelGGL(fn, dim3(cus * per_cu), dim3(kThreads), NS * P::STAGE, stream, a);
+  const int per_cu = 2 * P::LDS <= 160 * 1024 ? 2 : 1;
+  hipLaunchKernelGGL(fn, dim3(cus * per_cu), dim3(kThreads), P::LDS, stream, a);
   return ce_launched();
 }
 
@@ -1065,11 +1112,11 @@ static int launch_dh(const CeArgs& a, const CePlan& p, hipStream_t stream) {
   using P = HiddenGrad<T, BM, BN, WM, NS, SHIFT>;
   static bool set[16];
   auto* fn = &k_ce_dh<T, BM, BN, WM, NS, SHIFT>;
-  const int rc = ce_lds(fn, NS * P::STAGE, set);
+  const int rc = ce_lds(fn, P::LDS, set);
   if (rc != MXS_OK) return rc;
   const int rows = a.rows < a.T ? a.rows : a.T;
   const int nx = (a.D + BN - 1) / BN, ny = (rows + BM - 1) / BM;
-  hipLaunchKernelGGL(fn, dim3(nx * ny * p.splits), dim3(kThreads), NS * P::STAGE, stream, a, nx,
+  hipLaunchKernelGGL(fn, dim3(nx * ny * p.splits), dim3(kThreads), P::LDS, stream, a, nx,
                      ny);
   return ce_launched();
 }
@@ -1079,9 +1126,9 @@ static int launch_dw(const CeArgs& a, int cus, hipStream_t stream) {
   using P = TableGrad<T, BN, NS>;
   static bool set[16];
   auto* fn = &k_ce_dw<T, BN, NS>;
-  const int rc = ce_lds(fn, NS * P::STAGE, set);
+  const int rc = ce_lds(fn, P::LDS, set);
   if (rc != MXS_OK) return rc;
-  hipLaunchKernelGGL(fn, dim3(cus), dim3(kThreads), NS * P::STAGE, stream, a);
+  hipLaunchKernelGGL(fn, dim3(cus), dim3(kThreads), P::LDS, stream, a);
   return ce_launched();
 }
 
@@ -1094,22 +1141,22 @@ static int launch_dw(const CeArgs& a, int cus, hipStream_t stream) {
 template <typename T, bool KEEP>
 static int logits_of(const CeArgs& a, const CePlan& p, int cus, hipStream_t stream) {
   switch (p.bm) {
-    case 32: return launch_logits<T, 32, 1, 4, KEEP>(a, cus, stream);
-    case 64: return launch_logits<T, 64, 2, 3, KEEP>(a, cus, stream);
-    case 128: return launch_logits<T, 128, 2, 3, KEEP>(a, cus, stream);
-    default: return launch_logits<T, 256, 4, 2, KEEP>(a, cus, stream);
+    case 32: return launch_logits<T, 32, 1, 5, KEEP>(a, cus, stream);
+    case 64: return launch_logits<T, 64, 2, 5, KEEP>(a, cus, stream);
+    case 128: return launch_logits<T, 128, 2, 5, KEEP>(a, cus, stream);
+    default: return launch_logits<T, 256, 4, 4, KEEP>(a, cus, stream);
   }
 }
 
 template <typename T, bool SHIFT>
 static int dh_of(const CeArgs& a, const CePlan& p, hipStream_t stream) {
   if (p.dh_bm == 64)
-    return p.dh_bn == 256 ? launch_dh<T, 64, 256, 2, 3, SHIFT>(a, p, stream)
-                          : launch_dh<T, 64, 128, 2, 3, SHIFT>(a, p, stream);
+    return p.dh_bn == 256 ? launch_dh<T, 64, 256, 2, 6, SHIFT>(a, p, stream)
+                          : launch_dh<T, 64, 128, 2, 8, SHIFT>(a, p, stream);
   switch (p.dh_bn) {
-    case 256: return launch_dh<T, 256, 256, 4, 2, SHIFT>(a, p, stream);
-    case 192: return launch_dh<T, 256, 192, 4, 2, SHIFT>(a, p, stream);
-    default: return launch_dh<T, 256, 128, 4, 3, SHIFT>(a, p, stream);
+    case 256: return launch_dh<T, 256, 256, 4, 4, SHIFT>(a, p, stream);
+    case 192: return launch_dh<T, 256, 192, 4, 5, SHIFT>(a, p, stream);
+    default: return launch_dh<T, 256, 128, 4, 6, SHIFT>(a, p, stream);
   }
 }
 
@@ -1139,7 +1186,7 @@ static int run_ce(CeArgs a, const CePlan& p, int cus, hipStream_t stream) {
       const int tbs = a.rows / 32, ys = 4096 / tbs + 1;
       hipLaunchKernelGGL(k_ce_dz<T>, dim3(tbs, ys), dim3(256), 0, stream, a);
       CE_TRY(ce_launched());
-      CE_TRY((launch_dw<T, 256, 2>(a, cus, stream)));
+      CE_TRY((launch_dw<T, 256, 4>(a, cus, stream)));
     }
     if (a.dh) {
       CE_TRY(shift ? (dh_of<T, true>(a, p, stream)) : (dh_of<T, false>(a, p, stream)));
@@ -1160,7 +1207,7 @@ static int run_ce(CeArgs a, const CePlan& p, int cus, hipStream_t stream) {
 
 static int ce_sizes(int T, int V, int D) {
   if (T < 0 || V <= 0 || D <= 0) return MXS_ERR_ARG;
-  return D % kK || D > 65536 || T > (1 << 24) || V > (1 << 28) ? MXS_ERR_SIZE : MXS_OK;
+  return D % 64 || D > 65536 || T > (1 << 24) || V > (1 << 28) ? MXS_ERR_SIZE : MXS_OK;
 }
 
 }  // namespace mxs
