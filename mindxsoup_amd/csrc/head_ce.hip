@@ -431,6 +431,7 @@ __device__ __forceinline__ int xcd_place(int b, int n) {
 // BM rows x kVocabTile columns a tile, WM x (8 / WM) waves.
 template <typename T, int BM, int WM, int NS_, bool KEEP>
 struct Logits {
+  static constexpr bool RANGE = BM < 256;
   static constexpr int BN = kVocabTile, WN = kWaves / WM, NS = NS_;
   static constexpr int TM = BM / 32 / WM, TN = BN / 32 / WN;
   static constexpr int COLS = 32 * TN;  // columns of a wave: one block of statistics
@@ -438,8 +439,8 @@ struct Logits {
   using B = RowTile<BN>;
   static constexpr int STAGE = A::BYTES + B::BYTES, NCP = A::N + B::N;
   // Labels of a tile's rows, copied with its first step: a load in the epilogue would wait for
-  // every copy before it.  The copies are at most three tiles ahead (two steps a tile at least).
-  static constexpr int SLOTS = 4, LDS = NS * STAGE + SLOTS * 1024;
+  // every copy before it.  With two steps a tile at least the copies are (NS + 1) / 2 tiles ahead.
+  static constexpr int SLOTS = NS > 6 ? 8 : 4, LDS = NS * STAGE + SLOTS * 1024;
   static_assert((NS + 1) / 2 < SLOTS && A::kEven + B::kEven > 0, "label slots, copies per wave");
   static constexpr int STORES = KEEP ? TM * TN * 2 : 0;  // at least: 16 bytes a lane is the widest
   const CeArgs& a;
@@ -447,6 +448,7 @@ struct Logits {
   A ca;
   B cb;
   int wave, lane, mt, wm0, wn0, m_copy;
+  int first_col, end;  // of the workgroup's columns, where it has a range of its own
   bool lean;
 
   __device__ __forceinline__ Logits(const CeArgs& args, const char* lds) : a(args), smem(lds) {
@@ -462,17 +464,23 @@ struct Logits {
   __device__ __forceinline__ int place(int q) const {
     return q * (int)gridDim.x + xcd_place((int)blockIdx.x, (int)gridDim.x);
   }
-  __device__ __forceinline__ void coords(int at, int& vt, int& m) const {
-    const int g = at / (4 * mt), rest = at - g * 4 * mt;
-    vt = g * 4 + (rest & 3);
-    m = rest >> 2;
+  // RANGE: there is one row tile only, and the table is shared out evenly, in blocks of COLS
+  // columns; a workgroup's last tile is then partly empty, and reads no more than its columns.
+  __device__ __forceinline__ void coords(int q, int& v0, int& m) const {
+    if constexpr (RANGE) {
+      v0 = first_col + q * BN;
+      m = 0;
+    } else {
+      const int at = place(q), g = at / (4 * mt), rest = at - g * 4 * mt;
+      v0 = (g * 4 + (rest & 3)) * BN;
+      m = rest >> 2;
+    }
   }
   __device__ __forceinline__ void enter(int q) {
-    int vt;
-    coords(place(q), vt, m_copy);
-    const int last = a.V - 1, v0 = min(vt * BN, last);
+    int v0;
+    coords(q, v0, m_copy);
     ca.tile(a.hc, a.D, a.row0 + m_copy * BM, a.row0 + a.rows - 1, wave, lane);
-    cb.tile(a.w, a.ldw, v0, last, wave, lane);
+    cb.tile(a.w, a.ldw, min(v0, end - 1), end - 1, wave, lane);
   }
   __device__ __forceinline__ void copy(uint32_t lds, int q, int k, int c) const {
     // one wave's copy more than NCP: the counted waits then wait for more, not for less
@@ -497,10 +505,11 @@ struct Logits {
 
   // acc[i][j][r]: row 32 i + lane % 32, column 32 j + 8 (r / 4) + 4 (lane / 32) + r % 4.
   __device__ __forceinline__ bool done(int q, float16_t (&acc)[TM][TN]) const {
-    int vt, m;
-    coords(place(q), vt, m);
-    const int v0 = vt * BN + wn0;
-    if (vt * BN >= a.V) return false;
+    int v0, m;
+    coords(q, v0, m);
+    if (v0 >= a.V) return false;
+    v0 += wn0;
+    if (RANGE && v0 >= end) return false;  // another workgroup's
     const int h = lane >> 5;
     if (v0 + COLS > a.V) {  // columns past the vocabulary
 #pragma unroll
@@ -572,9 +581,20 @@ __global__ __launch_bounds__(kThreads) void k_ce_logits(CeArgs a) {
   using P = Logits<T, BM, WM, NS, KEEP>;
   P p(a, smem);
   p.mt = (piece_rows(a) + BM - 1) / BM;
-  const int vt = (a.V + P::BN - 1) / P::BN, places = (vt + 3) / 4 * 4 * p.mt;
   const int g = (int)gridDim.x, wg = p.place(0);
-  const int tiles = wg < places ? (places - wg + g - 1) / g : 0;
+  int tiles = 0;
+  p.first_col = 0, p.end = a.V;
+  if constexpr (P::RANGE) {
+    const int blocks = (a.V + P::COLS - 1) / P::COLS, per = (blocks + g - 1) / g * P::COLS;
+    p.first_col = wg * per;
+    if (p.mt && p.first_col < a.V) {
+      p.end = min(p.first_col + per, a.V);
+      tiles = (p.end - p.first_col + P::BN - 1) / P::BN;
+    }
+  } else {
+    const int vt = (a.V + P::BN - 1) / P::BN, places = (vt + 3) / 4 * 4 * p.mt;
+    tiles = wg < places ? (places - wg + g - 1) / g : 0;
+  }
   if (tiles > 0) stream_tiles<T, P::TM, P::TN>(p, smem, tiles, a.D / kK);
 }
 
@@ -689,7 +709,7 @@ __global__ __launch_bounds__(256) void k_ce_dz(CeArgs a) {
 #pragma unroll
     for (int r = 0; r < 8; r += 2) {
       float lo = 0.0f, hi = 0.0f;
-      if (row < n) {
+      if (row < n && v0 < a.V) {
         const int v = v0 + 8 * (r >> 2) + 4 * h + (r & 3);
         lo = v == y ? at_label : (float)e[r] * w;
         hi = v + 1 == y ? at_label : (float)e[r + 1] * w;
@@ -1141,9 +1161,9 @@ static int launch_dw(const CeArgs& a, int cus, hipStream_t stream) {
 template <typename T, bool KEEP>
 static int logits_of(const CeArgs& a, const CePlan& p, int cus, hipStream_t stream) {
   switch (p.bm) {
-    case 32: return launch_logits<T, 32, 1, 5, KEEP>(a, cus, stream);
-    case 64: return launch_logits<T, 64, 2, 5, KEEP>(a, cus, stream);
-    case 128: return launch_logits<T, 128, 2, 5, KEEP>(a, cus, stream);
+    case 32: return launch_logits<T, 32, 1, 8, KEEP>(a, cus, stream);
+    case 64: return launch_logits<T, 64, 2, 7, KEEP>(a, cus, stream);
+    case 128: return launch_logits<T, 128, 2, 6, KEEP>(a, cus, stream);
     default: return launch_logits<T, 256, 4, 4, KEEP>(a, cus, stream);
   }
 }
