@@ -13,6 +13,9 @@ csrc/torch_ops.cpp (host C++ only, no device code) is compiled by g++ against to
 beside them and linked into mindxsoup_amd/libmxs_nf4_torch.so, which registers the
 torch.ops.mxs_nf4 operators and links libmxs_nf4.so from its own directory.
 
+csrc/py_lists.cpp is a small Python module over that library (mindxsoup_amd/_mxs_lists.so): the
+operators over lists of tensors, called with Python lists.
+
 Sources that issue global loads as inline asm (the ones calling vm_ready) are also compiled to
 device assembly, which isa_check verifies: no instruction may name a register whose load can
 still be in flight.  A finding fails the build.
@@ -22,6 +25,7 @@ import concurrent.futures
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -30,6 +34,8 @@ OBJ = os.path.join(CSRC, "_build")
 LIB = os.path.join(PKG, "libmxs_nf4.so")
 TORCH_SRC = os.path.join(CSRC, "torch_ops.cpp")
 TORCH_LIB = os.path.join(PKG, "libmxs_nf4_torch.so")
+PY_SRC = os.path.join(CSRC, "py_lists.cpp")
+PY_LIB = os.path.join(PKG, "_mxs_lists.so")
 PROBE_SRC = os.path.join(CSRC, "probe", "hbm_probe.hip")
 PROBE_LIB = os.path.join(PKG, "libmxs_probe.so")
 ARCH = "gfx950"
@@ -99,22 +105,22 @@ def _torch_flags():
     return compile_flags, link_flags
 
 
-def _compile_torch_ops():
-    obj = os.path.join(OBJ, "torch_ops.o")
-    r = subprocess.run(["g++", *_torch_flags()[0], "-c", TORCH_SRC, "-o", obj],
+def _compile_host(src, *flags):
+    obj = os.path.join(OBJ, os.path.basename(src)[:-4] + ".o")
+    r = subprocess.run(["g++", *_torch_flags()[0], *flags, "-c", src, "-o", obj],
                        capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"g++ failed on {TORCH_SRC}:\n{r.stderr}")
+        raise RuntimeError(f"g++ failed on {src}:\n{r.stderr}")
     return obj
 
 
-def _link_torch_ops(obj):
-    tmp = TORCH_LIB + ".tmp"
-    r = subprocess.run(["g++", "-shared", obj, "-o", tmp, *_torch_flags()[1]],
+def _link_host(obj, lib, *flags):
+    tmp = lib + ".tmp"
+    r = subprocess.run(["g++", "-shared", obj, "-o", tmp, *flags, *_torch_flags()[1]],
                        capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"link of {TORCH_LIB} failed:\n{r.stderr}")
-    os.replace(tmp, TORCH_LIB)
+        raise RuntimeError(f"link of {lib} failed:\n{r.stderr}")
+    os.replace(tmp, lib)
 
 
 def _link_hip(objs, lib):
@@ -130,21 +136,24 @@ def build(verbose=True):
     os.makedirs(OBJ, exist_ok=True)
     srcs = sources()
     asm_srcs = [s for s in srcs if "vm_ready(" in open(s).read()]
-    workers = min(len(srcs) + len(asm_srcs) + 2, max(1, (os.cpu_count() or 4)), 8)
+    workers = min(len(srcs) + len(asm_srcs) + 3, max(1, (os.cpu_count() or 4)), 8)
     with concurrent.futures.ThreadPoolExecutor(workers) as ex:
-        torch_obj = ex.submit(_compile_torch_ops)
+        torch_obj = ex.submit(_compile_host, TORCH_SRC)
+        py_obj = ex.submit(_compile_host, PY_SRC, "-I" + sysconfig.get_path("include"))
         probe_obj = ex.submit(_compile, PROBE_SRC)
         checks = [ex.submit(_check_asm, s) for s in asm_srcs]
         objs = list(ex.map(_compile, srcs))
         for c in checks:
             c.result()
         torch_obj = torch_obj.result()
+        py_obj = py_obj.result()
         probe_obj = probe_obj.result()
     _link_hip(objs, LIB)
     _link_hip([probe_obj], PROBE_LIB)
-    _link_torch_ops(torch_obj)
+    _link_host(torch_obj, TORCH_LIB)
+    _link_host(py_obj, PY_LIB, f"-L{PKG}", "-l:" + os.path.basename(TORCH_LIB), "-ltorch_python")
     if verbose:
-        print(f"built {LIB} from {len(srcs)} sources, {TORCH_LIB} and {PROBE_LIB}")
+        print(f"built {LIB} from {len(srcs)} sources, {TORCH_LIB}, {PY_LIB} and {PROBE_LIB}")
     return LIB
 
 

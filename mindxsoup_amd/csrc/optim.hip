@@ -2,8 +2,8 @@
 // step over many parameter tensors with its two states in fp32 or in 8 bits.
 //
 // All of it is bound by HBM: every gradient, parameter and state is read once and written once.
-// Tensors travel to a launch in its kernel arguments (pointers and sizes, at most 4 KB, so 88
-// fp32-state or 64 8-bit-state tensors a launch; 200 gradients of a norm), so a step copies
+// Tensors travel to a launch in its kernel arguments (pointers and sizes, at most 4 KB, so 86
+// fp32-state or 63 8-bit-state tensors a launch; 228 gradients of a norm), so a step copies
 // nothing to the device and can be captured: a workgroup finds its tensor by a binary search over
 // the first chunk of each.
 //
@@ -28,23 +28,38 @@ constexpr int kStepArgs = 3900;   // bytes of a launch's tensor table
 // The 8-bit dynamic map (Dettmers, arXiv 1511.04561), ascending: the signed one is the code book
 // of the nested absmax; the unsigned one has a bit more of fraction (2^(i+1) midpoints in decade
 // i instead of 2^i and their negatives).  Both hold 0 and 1.
+//
+// The nearest code of x, relative to its block's largest magnitude, is the number of borders
+// (midpoints of neighbours) below it.  The leading 16 bits of |x| plus an offset pick an interval
+// that holds one border at most, and whose ends no border comes near (within 2^-14, relative: many
+// borders lie on fractions of few bits, where the intervals would end without the offset): the
+// code is the count of borders below the interval, and one more if its border is below x.  In
+// fp32 that is sure unless x is within 2^-20 of the border, relative; then, one value in 10^4 or
+// so, it is decided in fp64, where border times scale is exact.
+constexpr uint32_t kKeyOffset = 0xa8f0;
+constexpr int kKeyBase = (0x34000000 + kKeyOffset) >> 16;  // of 2^-23: no border is nearer to 0
+constexpr int kKeys = ((0x3f800000 + kKeyOffset) >> 16) - kKeyBase + 1;  // up to 1
+
+constexpr float key_end(int k) {  // where interval k begins
+  return __builtin_bit_cast(float, ((uint32_t)(kKeyBase + k) << 16) - kKeyOffset);
+}
+
 struct Book {
-  float value[256];
-  double border[256];  // border[c]: a value above it is nearer to code c + 1; [255] is infinite
-  // codes to start the search from, by the leading 6 bits of fraction and the exponent of |x|
-  uint8_t pos[1474], neg[1474];
+  double value[256];
+  float border[256];  // border[c]: a value above it is nearer to code c + 1; [255] is infinite
+  uint8_t pos[kKeys + 1], neg[kKeys + 1];  // borders below the interval of +|x| and of -|x|
 };
 
-constexpr int kKeyBase = 104 << 6;          // 2^-23: no border lies between 0 and it
-constexpr int kKeys = ((127 - 104) << 6) + 1;  // up to 1
-constexpr int kBookSteps = 3;               // borders that a key's interval can hold, and slack
+struct Border64 {
+  double at[256];
+};
 
 constexpr Book make_book(bool is_signed) {
   Book b{};
   constexpr double decade[7] = {1e-6, 1e-5, 1e-4, 1e-3, 1e-2, 1e-1, 1.0};
   int at = is_signed ? 127 : 0;  // index of zero
   const int zero = at;
-  b.value[at++] = 0.0f;
+  b.value[at++] = 0.0;
   for (int i = 0; i < 7; i++) {
     const int n = is_signed ? 1 << i : 2 << i;
     for (int j = 0; j < n; j++) {
@@ -55,60 +70,66 @@ constexpr Book make_book(bool is_signed) {
       b.value[at++] = v;
     }
   }
-  b.value[255] = 1.0f;
-  for (int c = 0; c < 255; c++) b.border[c] = ((double)b.value[c] + (double)b.value[c + 1]) / 2;
-  b.border[255] = __builtin_huge_val();
-  // Interval k of |x|: [lo, hi).  The start is the number of borders surely below x; a hair of
-  // slack covers the rounding of x to fp32 before its key is taken.
-  double lo = 0.0, scale = 1.0 / (1 << 23);
+  b.value[255] = 1.0;
+  for (int c = 0; c < 255; c++) b.border[c] = (float)((b.value[c] + b.value[c + 1]) / 2);
+  b.border[255] = __builtin_huge_valf();
   int c = 0;
   for (int k = 0; k < kKeys; k++) {
-    const double hi = scale * (1.0 + ((k & 63) + 1) / 64.0);
-    while (b.border[c] < lo * (1 - 1e-6)) c++;
+    while (k > 0 && c < 255 && b.border[c] < key_end(k)) c++;
+    if (k == 0) c = zero;  // borders below 0
     b.pos[k] = (uint8_t)c;
-    int d = is_signed && c < 254 ? 254 - c : 0;  // symmetric borders but for the one below 1
-    while (d > 0 && b.border[d - 1] >= -hi * (1 + 1e-6)) d--;
+    int d = zero;
+    while (d > 0 && b.border[d - 1] >= -key_end(k + 1)) d--;
     b.neg[k] = (uint8_t)d;
-    lo = hi;
-    if ((k & 63) == 63) scale *= 2;
   }
   return b;
 }
 
-// Whether kBookSteps upward steps from every start reach the code of every x of the interval.
-constexpr bool book_ok(const Book& b, bool is_signed) {
-  double lo = 0.0, scale = 1.0 / (1 << 23);
-  for (int k = 0; k < kKeys; k++) {
-    const double hi = scale * (1.0 + ((k & 63) + 1) / 64.0);
-    if (b.pos[k] && b.border[b.pos[k] - 1] >= lo) return false;
-    const int p = b.pos[k] + kBookSteps;
-    if (p < 255 && !(b.border[p] >= hi * (1 + 1e-6)) && k + 1 < kKeys) return false;
-    if (is_signed) {
-      if (b.neg[k] > 127 || (b.neg[k] && b.border[b.neg[k] - 1] >= -hi)) return false;
-      const int n = b.neg[k] + kBookSteps;
-      if (n < 255 && !(b.border[n] >= -lo * (1 - 1e-6))) return false;
+constexpr Border64 make_borders(const Book& b) {
+  Border64 r{};
+  for (int c = 0; c < 255; c++) r.at[c] = (b.value[c] + b.value[c + 1]) / 2;  // 25 bits: exact
+  r.at[255] = __builtin_huge_val();
+  return r;
+}
+
+// One border at most in an interval of either sign, and none within 2^-14 of its ends, relative.
+constexpr bool book_ok(const Book& b, int zero) {
+  for (int side = 0; side < 2; side++) {
+    int c = side ? zero - 1 : zero;  // outwards from 0
+    for (int k = 0; k < kKeys; k++) {
+      int in = 0;
+      const double lo = key_end(k), hi = key_end(k + 1);
+      for (; c >= 0 && c < 255; c += side ? -1 : 1) {
+        const double a = side ? -b.border[c] : b.border[c];
+        if (a > hi * (1 - 0x1p-14) && a < hi * (1 + 0x1p-14)) return false;
+        if (a < lo || a >= hi) break;
+        in++;
+      }
+      if (in > 1) return false;
     }
-    lo = hi;
-    if ((k & 63) == 63) scale *= 2;
+    if (c >= 0 && c < 255) return false;
   }
   return true;
 }
 
 constexpr Book kSignedBook = make_book(true), kUnsignedBook = make_book(false);
-static_assert(book_ok(kSignedBook, true) && book_ok(kUnsignedBook, false), "steps of the search");
+static_assert(book_ok(kSignedBook, 127) && book_ok(kUnsignedBook, 0), "intervals of the search");
 __device__ __constant__ static const Book kBooks[2] = {kSignedBook, kUnsignedBook};
+__device__ __constant__ static const Border64 kBorders[2] = {make_borders(kSignedBook),
+                                                             make_borders(kUnsignedBook)};
 
-// The code whose value times `top` is nearest to x (the lower one of two as near): the number of
-// borders below x / top.  A border has 25 bits and top 24, so their products are exact; inv,
-// about 1 / top, only picks where the search starts.
-__device__ __forceinline__ int nearest_code(const Book& b, double x, double top, double inv) {
-  const float f = (float)(x * inv);
-  int k = (int)((__builtin_bit_cast(uint32_t, f) & 0x7fffffffu) >> 17) - kKeyBase;
+// The code whose value times `top` is nearest to x (the lower one of two as near); xf is x rounded
+// to fp32, inv 1 / top within two roundings (0 for a block of zeros).
+__device__ __forceinline__ int nearest_code(const Book& b, const Border64& exact, double x,
+                                            float xf, double top, float inv) {
+  const float f = xf * inv;
+  int k = (int)(((__builtin_bit_cast(uint32_t, f) & 0x7fffffffu) + kKeyOffset) >> 16) - kKeyBase;
   k = min(max(k, 0), kKeys - 1);
-  int c = f < 0.0f ? b.neg[k] : b.pos[k];
-#pragma unroll
-  for (int s = 0; s < kBookSteps; s++) c += b.border[c] * top < x ? 1 : 0;
-  return c;
+  const int c = f < 0.0f ? b.neg[k] : b.pos[k];
+  const float at = b.border[c];
+  bool above = at < f;
+  if (fabsf(f - at) <= fabsf(at) * 0x1p-20f) above = exact.at[c] * top < x;
+  return c + (above ? 1 : 0);
 }
 
 // ---- element access ---------------------------------------------------------------------------
@@ -178,10 +199,6 @@ __device__ __forceinline__ void store8_codes(uint8_t* p, int64_t i, int64_t n, b
 
 // ---- tables -----------------------------------------------------------------------------------
 
-struct NormTensor {
-  const void* g;
-  int64_t n;
-};
 struct StepTensor {
   void* p;
   const void* g;
@@ -203,9 +220,19 @@ struct Table {
   int count;
 };
 
+// Gradients of one launch of the norm; a longer one than 2^31 values takes several entries.
+struct NormTable {
+  static constexpr int N = (kStepArgs - 8) / 17;
+  const void* g[N];
+  uint32_t n[N];
+  int start[N + 1];
+  uint8_t flags[N];
+  int count;
+};
+
 // The tensor of chunk `c` (uniform).
-template <typename T>
-__device__ __forceinline__ int tensor_of(const Table<T>& tab, int c) {
+template <typename Tab>
+__device__ __forceinline__ int tensor_of(const Tab& tab, int c) {
   int lo = 0, hi = tab.count;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -241,27 +268,32 @@ __device__ __forceinline__ double squares(const T* g, int64_t i0, int64_t n, boo
   return a[0] + a[1];
 }
 
-// Sums of squares per chunk, in fp64: the squares of any fp32 and their sums are then neither
+constexpr int kNormGroups = 2048;  // workgroups of a launch at most: eight a CU
+
+// Sums of squares per workgroup, in fp64: the squares of any fp32 and their sums are then neither
 // infinite nor lost, whatever their sizes.
-__global__ __launch_bounds__(256) void k_norm_chunks(Table<NormTensor> tab, double* partial) {
+__global__ __launch_bounds__(256) void k_norm_chunks(NormTable tab, double* partial) {
   __shared__ double s[4];
-  const int c = (int)blockIdx.x, i = tensor_of(tab, c);
-  const int64_t at = (int64_t)(c - tab.start[i]) * kNormChunk, n = tab.t[i].n;
-  const bool vec = tab.flags[i] & kVec;
-  double a;
-  switch (tab.flags[i] & (kVec - 1)) {
-    case MXS_DTYPE_F16: a = squares(static_cast<const _Float16*>(tab.t[i].g), at, n, vec); break;
-    case MXS_DTYPE_BF16: a = squares(static_cast<const __bf16*>(tab.t[i].g), at, n, vec); break;
-    default: a = squares(static_cast<const float*>(tab.t[i].g), at, n, vec);
+  double a = 0.0;
+  for (int c = (int)blockIdx.x; c < tab.start[tab.count]; c += (int)gridDim.x) {
+    const int i = tensor_of(tab, c);
+    const int64_t at = (int64_t)(c - tab.start[i]) * kNormChunk, n = tab.n[i];
+    const bool vec = tab.flags[i] & kVec;
+    switch (tab.flags[i] & (kVec - 1)) {
+      case MXS_DTYPE_F16: a += squares(static_cast<const _Float16*>(tab.g[i]), at, n, vec); break;
+      case MXS_DTYPE_BF16: a += squares(static_cast<const __bf16*>(tab.g[i]), at, n, vec); break;
+      default: a += squares(static_cast<const float*>(tab.g[i]), at, n, vec);
+    }
   }
   a = sum256(a, s);
-  if (threadIdx.x == 0) partial[c] = a;
+  if (threadIdx.x == 0) partial[blockIdx.x] = a;
 }
 
 __global__ __launch_bounds__(256) void k_norm_finish(const double* partial, int64_t n,
                                                      const float* grad_scale, float* out) {
   __shared__ double s[4];
   double a = 0.0;
+#pragma unroll 8
   for (int64_t i = threadIdx.x; i < n; i += 256) a += partial[i];
   a = sum256(a, s);
   if (threadIdx.x == 0) out[0] = (float)(sqrt(a) / (grad_scale ? (double)grad_scale[0] : 1.0));
@@ -299,6 +331,14 @@ __global__ void k_adamw_scalars(StepScalars* out, float* step, double lr, const 
   if (!skip) step[0] = t;
 }
 
+// m / (sqrt(v) root + eps) with the hardware's root and reciprocal, each within one step of fp32;
+// roots of values below 2^-96 are taken 2^48 times larger.
+__device__ __forceinline__ float ratio(float m, float v, float root, float eps) {
+  const bool low = v < 0x1p-96f;
+  const float r = __builtin_amdgcn_sqrtf(low ? v * 0x1p96f : v) * (low ? 0x1p-48f : 1.0f);
+  return m * __builtin_amdgcn_rcpf(r * root + eps);
+}
+
 constexpr int kStepChunk = 2048;  // values of a workgroup, fp32 states
 
 template <typename T>
@@ -318,7 +358,7 @@ __device__ __forceinline__ void step32(const StepTensor& t, int64_t i, bool vec,
     const float x = g[e] * coef;
     m[e] = b1 * m[e] + c1 * x;
     v[e] = b2 * v[e] + c2 * (x * x);
-    p[e] = p[e] * s.keep - s.size * m[e] / (sqrtf(v[e]) * s.root + eps);
+    p[e] = p[e] * s.keep - s.size * ratio(m[e], v[e], s.root, eps);
   }
   store8(tm, i, t.n, vec, m);
   store8(tv, i, t.n, vec, v);
@@ -357,18 +397,23 @@ __device__ __forceinline__ float max32(float x) {
 
 // New values x[8] of a block as codes and the block's scale.  A block with a value that is not
 // finite gets a NaN scale: all of its values are then NaN, as they are lost.
-__device__ __forceinline__ float encode(const Book& b, const double (&x)[8], int (&c)[8]) {
-  float top = 0.0f;
+__device__ __forceinline__ float encode(const Book& b, const Border64& exact,
+                                        const double (&x)[8], int (&c)[8]) {
+  float f[8], top = 0.0f;
 #pragma unroll
   for (int e = 0; e < 8; e++) {
-    const float a = fabsf((float)x[e]);
+    f[e] = (float)x[e];
+    const float a = fabsf(f[e]);
     top = (top > a || top != top) ? top : a;
   }
   top = max32(top);
   if (top == __builtin_inff()) top = __builtin_nanf("");
-  const double inv = top > 0.0f ? 1.0 / (double)top : 0.0;
+  // A scale below fp32's normal range has no fp32 reciprocal: both sides times 2^64 then.
+  const bool low = top < 0x1p-100f;
+  const float up = low ? 0x1p64f : 1.0f;
+  const float inv = top > 0.0f ? __builtin_amdgcn_rcpf(top * up) : 0.0f;
 #pragma unroll
-  for (int e = 0; e < 8; e++) c[e] = nearest_code(b, x[e], (double)top, inv);
+  for (int e = 0; e < 8; e++) c[e] = nearest_code(b, exact, x[e], f[e] * up, (double)top, inv);
   return top;
 }
 
@@ -396,11 +441,12 @@ __device__ __forceinline__ void step8(const StepTensor8& t, int64_t i, bool vec,
   for (int e = 0; e < 8; e++) {
     const double x = (double)g[e] * s.coef;
     const bool in = i + e < t.n;
-    m[e] = in ? (double)books[0].value[cm[e]] * sm * b1 + x * (1.0 - b1) : 0.0;
-    v[e] = in ? (double)books[1].value[cv[e]] * sv * b2 + (x * x) * (1.0 - b2) : 0.0;
-    p[e] = p[e] * s.keep - s.size * (float)m[e] / (sqrtf((float)v[e]) * s.root + eps);
+    m[e] = in ? books[0].value[cm[e]] * sm * b1 + x * (1.0 - b1) : 0.0;
+    v[e] = in ? books[1].value[cv[e]] * sv * b2 + (x * x) * (1.0 - b2) : 0.0;
+    p[e] = p[e] * s.keep - s.size * ratio((float)m[e], (float)v[e], s.root, eps);
   }
-  const float topm = encode(books[0], m, cm), topv = encode(books[1], v, cv);
+  const float topm = encode(books[0], kBorders[0], m, cm);
+  const float topv = encode(books[1], kBorders[1], v, cv);
   if (live) {
     store8(tp, i, t.n, vec, p);
     store8_codes(tm, i, t.n, vec, cm);
@@ -440,21 +486,36 @@ __global__ __launch_bounds__(256) void k_adamw8(Table<StepTensor8> tab,
   }
 }
 
-// The values that codes stand for: book value times scale, rounded once.
+// The values that codes stand for: book value times scale, rounded once.  Four values a lane, so
+// that a wave's store is 1 KB in one piece; nothing is read again, so loads and stores pass the
+// caches by.
 __global__ __launch_bounds__(256) void k_state_values(const uint8_t* codes, const float* scale,
-                                                      float* out, int64_t n, int book, bool vec) {
+                                                      float* out, int64_t n, int book, int vec) {
   __shared__ float value[256];
-  value[threadIdx.x] = kBooks[book].value[threadIdx.x];
+  value[threadIdx.x] = (float)kBooks[book].value[threadIdx.x];
   __syncthreads();
-  const int64_t stride = (int64_t)gridDim.x * 2048;
-  for (int64_t i = (int64_t)blockIdx.x * 2048 + threadIdx.x * 8; i < n; i += stride) {
-    int c[8];
-    float x[8];
-    load8_codes(codes, i, n, vec, c);
-    const float s = scale[i / kStateBlock];
+  const int64_t i0 = (int64_t)blockIdx.x * 4096 + threadIdx.x * 4;
+  if (vec && i0 - threadIdx.x * 4 + 4096 <= n) {
+    uint32_t c[4];
+    float s[4];
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = value[c[e]] * s;
-    store8(out, i, n, vec, x);
+    for (int u = 0; u < 4; u++) {
+      c[u] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(codes + i0 + u * 1024));
+      s[u] = scale[(i0 + u * 1024) / kStateBlock];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      float4_t x;
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] = value[(c[u] >> (8 * e)) & 255] * s[u];
+      __builtin_nontemporal_store(x, reinterpret_cast<float4_t*>(out + i0 + u * 1024));
+    }
+  } else {
+    for (int u = 0; u < 4; u++)
+      for (int e = 0; e < 4; e++) {
+        const int64_t i = i0 + u * 1024 + e;
+        if (i < n) out[i] = value[codes[i]] * scale[i / kStateBlock];
+      }
   }
 }
 
@@ -526,20 +587,39 @@ int mxs_grad_norm(int count, const void* const* grads, const int64_t* sizes, con
   }
   double* partial = static_cast<double*>(workspace);
   if ((uintptr_t)workspace % 8) return MXS_ERR_ALIGN;
-  const int rc = tables<NormTensor>(
-      count, sizes, kNormChunk,
-      [&](NormTensor& t, uint8_t& flags, int i) {
-        t = {grads[i], sizes[i]};
-        flags = (uint8_t)(dtypes[i] | (on16(grads[i]) ? kVec : 0));
-      },
-      [&](const Table<NormTensor>& tab, int chunks, int64_t before) {
-        hipLaunchKernelGGL(k_norm_chunks, dim3(chunks), dim3(256), 0, stream, tab,
-                           partial + before);
-        return launched();
-      });
+  NormTable tab;
+  int64_t groups = 0;
+  tab.count = 0, tab.start[0] = 0;
+  auto flush = [&]() {
+    const int chunks = tab.start[tab.count], grid = chunks < kNormGroups ? chunks : kNormGroups;
+    if (grid == 0) return MXS_OK;
+    hipLaunchKernelGGL(k_norm_chunks, dim3(grid), dim3(256), 0, stream, tab, partial + groups);
+    groups += grid;
+    tab.count = 0;
+    return launched();
+  };
+  for (int i = 0; i < count; i++) {
+    const int64_t most = (int64_t)1 << 31;
+    const int width = dtypes[i] == MXS_DTYPE_F32 ? 4 : 2;
+    for (int64_t at = 0; at < sizes[i]; at += most) {
+      const int64_t n = sizes[i] - at < most ? sizes[i] - at : most;
+      const int chunks = (int)((n + kNormChunk - 1) / kNormChunk);
+      if (tab.count == NormTable::N || tab.start[tab.count] > (1 << 30)) {
+        const int rc = flush();
+        if (rc != MXS_OK) return rc;
+      }
+      const char* g = static_cast<const char*>(grads[i]) + at * width;
+      tab.g[tab.count] = g;
+      tab.n[tab.count] = (uint32_t)n;
+      tab.flags[tab.count] = (uint8_t)(dtypes[i] | (on16(g) ? kVec : 0));
+      tab.start[tab.count + 1] = tab.start[tab.count] + chunks;
+      tab.count++;
+    }
+  }
+  const int rc = flush();
   if (rc != MXS_OK) return rc;
-  hipLaunchKernelGGL(k_norm_finish, dim3(1), dim3(256), 0, stream, partial,
-                     norm_chunks(count, sizes), grad_scale, out);
+  hipLaunchKernelGGL(k_norm_finish, dim3(1), dim3(256), 0, stream, partial, groups, grad_scale,
+                     out);
   return launched();
 }
 
@@ -604,11 +684,16 @@ int mxs_state_values(const void* codes, const float* scale, int64_t n, int is_si
   if (n < 0) return MXS_ERR_ARG;
   if (n == 0) return MXS_OK;
   if (!codes || !scale || !out) return MXS_ERR_ARG;
-  const int64_t chunks = (n + 2047) / 2048;
-  hipLaunchKernelGGL(k_state_values, dim3((unsigned)(chunks < 8192 ? chunks : 8192)), dim3(256),
-                     0, stream, static_cast<const uint8_t*>(codes), scale, out, n,
-                     is_signed ? 0 : 1, on16(codes) && on16(out));
-  return launched();
+  const int vec = (uintptr_t)codes % 4 == 0 && on16(out);
+  for (int64_t at = 0; at < n; at += (int64_t)1 << 40) {  // a grid's 32 bits of workgroups
+    const int64_t some = n - at < ((int64_t)1 << 40) ? n - at : (int64_t)1 << 40;
+    hipLaunchKernelGGL(k_state_values, dim3((unsigned)((some + 4095) / 4096)), dim3(256), 0,
+                       stream, static_cast<const uint8_t*>(codes) + at, scale + at / kStateBlock,
+                       out + at, some, is_signed ? 0 : 1, vec);
+    const int rc = launched();
+    if (rc != MXS_OK) return rc;
+  }
+  return MXS_OK;
 }
 
 }  // extern "C"

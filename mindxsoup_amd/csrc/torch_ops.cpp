@@ -41,6 +41,7 @@
 #include <vector>
 
 #include "mxs_nf4.h"
+#include "step_lists.h"
 
 namespace {
 
@@ -1607,11 +1608,11 @@ void adamw_step_cuda(TensorList params, TensorList grads, TensorList avgs, Tenso
   std::vector<int64_t> sizes(n);
   std::vector<int> dtypes(n);
   using Range = std::pair<uintptr_t, uintptr_t>;
-  std::vector<Range> written;
-  written.reserve(5 * n + 1);
-  auto writes = [&](const Tensor& t) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
-    if (t.numel()) written.push_back({at, at + t.nbytes()});
+  std::array<std::vector<Range>, 5> lists;  // memory that the step writes
+  for (auto& l : lists) l.reserve(n);
+  auto writes = [&](int list, const Tensor& t, const void* data) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(data);
+    if (t.numel()) lists[list].push_back({at, at + t.nbytes()});
   };
   const auto state = bits8 ? at::kByte : at::kFloat;
   for (size_t i = 0; i < n; i++) {
@@ -1642,8 +1643,8 @@ void adamw_step_cuda(TensorList params, TensorList grads, TensorList avgs, Tenso
                     t->scalar_type(), " ", t->sizes());
       ms[i] = avg_scales[i].data_ptr<float>();
       vs[i] = avg_sq_scales[i].data_ptr<float>();
-      writes(avg_scales[i]);
-      writes(avg_sq_scales[i]);
+      writes(3, avg_scales[i], ms[i]);
+      writes(4, avg_sq_scales[i], vs[i]);
     }
     const bool direct = gi.strides() == pi.strides();
     if (!direct) {
@@ -1655,10 +1656,20 @@ void adamw_step_cuda(TensorList params, TensorList grads, TensorList avgs, Tenso
     m[i] = mi.data_ptr();
     v[i] = vi.data_ptr();
     sizes[i] = pi.numel();
-    for (const Tensor* t : {&pi, &mi, &vi}) writes(*t);
+    writes(0, pi, p[i]);
+    writes(1, mi, m[i]);
+    writes(2, vi, v[i]);
   }
-  writes(step);
-  std::sort(written.begin(), written.end());
+  // merged into one ascending list (a list that an allocator or a flat buffer handed out in
+  // order is sorted already)
+  writes(0, step, step.data_ptr());
+  std::vector<Range> written, merged;
+  for (auto& l : lists) {
+    if (!std::is_sorted(l.begin(), l.end())) std::sort(l.begin(), l.end());
+    merged.resize(written.size() + l.size());
+    std::merge(written.begin(), written.end(), l.begin(), l.end(), merged.begin());
+    written.swap(merged);
+  }
   for (size_t i = 1; i < written.size(); i++)
     TORCH_CHECK(written[i - 1].second <= written[i].first,
                 "two of the tensors that the step writes overlap");
@@ -1706,6 +1717,22 @@ Tensor state_values_cuda(const Tensor& codes, const Tensor& scale, bool is_signe
 }
 
 }  // namespace
+
+namespace mxs_lists {
+
+Tensor grad_norm(TensorList grads, const OptTensor& grad_scale) {
+  return grad_norm_cuda(grads, grad_scale);
+}
+
+void adamw_step(TensorList params, TensorList grads, TensorList avgs, TensorList avg_sqs,
+                TensorList avg_scales, TensorList avg_sq_scales, const Tensor& step,
+                const StepOptions& o) {
+  adamw_step_cuda(params, grads, avgs, avg_sqs, avg_scales, avg_sq_scales, step, o.lr, o.lr_dev,
+                  o.beta1, o.beta2, o.eps, o.weight_decay, o.norm, o.max_norm, o.grad_scale,
+                  o.found_inf);
+}
+
+}  // namespace mxs_lists
 
 TORCH_LIBRARY(mxs_nf4, m) {
   m.def("dequant(Tensor packed, Tensor? absmax8, Tensor? code, Tensor? absmax2, Tensor? offset, "

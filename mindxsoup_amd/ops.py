@@ -49,6 +49,24 @@ def load():
     return _ops
 
 
+_lists = None
+
+
+def lists():
+    """The Python module of the operators over lists of tensors (csrc/py_lists.cpp): grad_norm and
+    adamw_step as torch.ops.mxs_nf4 has them, on Python lists."""
+    global _lists
+    if _lists is None:
+        load()
+        try:
+            from . import _mxs_lists
+        except ImportError as e:
+            raise _lib.MxsLibraryError(
+                f"_mxs_lists.so is not built ({e}): run `python -m mindxsoup_amd.build`") from e
+        _lists = _mxs_lists
+    return _lists
+
+
 def nf4(packed, state):
     """The five NF4 operand tensors the ops take after the input: packed bytes, absmax (u8),
     the second-level code book, the second-level absmax and the offset."""

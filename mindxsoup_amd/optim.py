@@ -37,8 +37,7 @@ def grad_norm(grads, grad_scale=None):
     grads = list(grads)
     if not grads:
         raise ValueError("grad_norm takes at least one gradient")
-    _on_gpu(grads[:1], "grad_norm")
-    return ops.load().grad_norm(grads, grad_scale)
+    return ops.lists().grad_norm(grads, grad_scale)
 
 
 @torch.no_grad()
@@ -73,10 +72,10 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
         raise ValueError(f"eps {eps}, weight_decay {weight_decay}, max_norm {max_norm}")
     lr_dev = lr if isinstance(lr, torch.Tensor) else None
     ms, vs = ([], []) if scales is None else map(list, scales)
-    ops.load().adamw_step(params, grads, exp_avgs, exp_avg_sqs, ms, vs, step,
-                          0.0 if lr_dev is not None else float(lr), lr_dev, float(b1), float(b2),
-                          float(eps), float(weight_decay), norm,
-                          1.0 if max_norm is None else float(max_norm), grad_scale, found_inf)
+    ops.lists().adamw_step(params, grads, exp_avgs, exp_avg_sqs, ms, vs, step,
+                           0.0 if lr_dev is not None else float(lr), lr_dev, float(b1),
+                           float(b2), float(eps), float(weight_decay), norm,
+                           1.0 if max_norm is None else float(max_norm), grad_scale, found_inf)
 
 
 @torch.no_grad()

@@ -320,7 +320,7 @@ def test_refusals(cuda):
     with pytest.raises(RuntimeError, match="overlap"):
         p = x()
         run([p, p], [x(), x()], [x(), x()], [x(), x()], step, lr=0.1)
-    with pytest.raises(RuntimeError, match="must be on"):
+    with pytest.raises(ValueError, match="GPU tensor"):
         run([x()], [torch.zeros(8)], [x()], [x()], step, lr=0.1)
     for kw in (dict(norm=step), dict(max_norm=1.0), dict(betas=(1.0, 0.5)), dict(eps=-1.0),
                dict(weight_decay=-1.0), dict(norm=step, max_norm=0.0)):
