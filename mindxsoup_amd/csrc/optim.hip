@@ -47,7 +47,7 @@ constexpr float key_end(int k) {  // where interval k begins
 struct Book {
   double value[256];
   float border[256];  // border[c]: a value above it is nearer to code c + 1; [255] is infinite
-  uint8_t pos[kKeys + 1], neg[kKeys + 1];  // borders below the interval of +|x| and of -|x|
+  uint8_t below[2 * kKeys + 2];  // borders below the interval of |x|, and of -|x| from kKeys on
 };
 
 struct Border64 {
@@ -77,10 +77,10 @@ constexpr Book make_book(bool is_signed) {
   for (int k = 0; k < kKeys; k++) {
     while (k > 0 && c < 255 && b.border[c] < key_end(k)) c++;
     if (k == 0) c = zero;  // borders below 0
-    b.pos[k] = (uint8_t)c;
+    b.below[k] = (uint8_t)c;
     int d = zero;
     while (d > 0 && b.border[d - 1] >= -key_end(k + 1)) d--;
-    b.neg[k] = (uint8_t)d;
+    b.below[kKeys + k] = (uint8_t)d;
   }
   return b;
 }
@@ -120,15 +120,18 @@ __device__ __constant__ static const Border64 kBorders[2] = {make_borders(kSigne
 
 // The code whose value times `top` is nearest to x (the lower one of two as near); xf is x rounded
 // to fp32, inv 1 / top within two roundings (0 for a block of zeros).
-__device__ __forceinline__ int nearest_code(const Book& b, const Border64& exact, double x,
-                                            float xf, double top, float inv) {
+template <bool SIGNED>
+__device__ __forceinline__ int nearest_code(const Book& b, double x, float xf, float top,
+                                            float inv) {
   const float f = xf * inv;
   int k = (int)(((__builtin_bit_cast(uint32_t, f) & 0x7fffffffu) + kKeyOffset) >> 16) - kKeyBase;
   k = min(max(k, 0), kKeys - 1);
-  const int c = f < 0.0f ? b.neg[k] : b.pos[k];
+  if (SIGNED && f < 0.0f) k += kKeys;
+  const int c = b.below[k];
   const float at = b.border[c];
   bool above = at < f;
-  if (fabsf(f - at) <= fabsf(at) * 0x1p-20f) above = exact.at[c] * top < x;
+  if (fabsf(f - at) <= fabsf(at) * 0x1p-20f)
+    above = kBorders[SIGNED ? 0 : 1].at[c] * (double)top < x;
   return c + (above ? 1 : 0);
 }
 
@@ -268,7 +271,7 @@ __device__ __forceinline__ double squares(const T* g, int64_t i0, int64_t n, boo
   return a[0] + a[1];
 }
 
-constexpr int kNormGroups = 2048;  // workgroups of a launch at most: eight a CU
+constexpr int kNormGroups = 16384;  // workgroups of a launch at most
 
 // Sums of squares per workgroup, in fp64: the squares of any fp32 and their sums are then neither
 // infinite nor lost, whatever their sizes.
@@ -289,14 +292,20 @@ __global__ __launch_bounds__(256) void k_norm_chunks(NormTable tab, double* part
   if (threadIdx.x == 0) partial[blockIdx.x] = a;
 }
 
-__global__ __launch_bounds__(256) void k_norm_finish(const double* partial, int64_t n,
-                                                     const float* grad_scale, float* out) {
-  __shared__ double s[4];
+__global__ __launch_bounds__(1024) void k_norm_finish(const double* partial, int64_t n,
+                                                      const float* grad_scale, float* out) {
+  __shared__ double s[16];
   double a = 0.0;
-#pragma unroll 8
-  for (int64_t i = threadIdx.x; i < n; i += 256) a += partial[i];
-  a = sum256(a, s);
-  if (threadIdx.x == 0) out[0] = (float)(sqrt(a) / (grad_scale ? (double)grad_scale[0] : 1.0));
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < n; i += 1024) a += partial[i];
+#pragma unroll
+  for (int o = 32; o; o >>= 1) a += __shfl_xor(a, o);
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = a;
+  __syncthreads();
+  if (threadIdx.x) return;
+  a = 0.0;
+  for (int w = 0; w < 16; w++) a += s[w];
+  out[0] = (float)(sqrt(a) / (grad_scale ? (double)grad_scale[0] : 1.0));
 }
 
 // ---- AdamW ------------------------------------------------------------------------------------
@@ -385,39 +394,45 @@ __global__ __launch_bounds__(256) void k_adamw(Table<StepTensor> tab, const Step
 
 constexpr int kStep8Chunk = 2048;  // values of a workgroup, 8-bit states: 8 blocks
 
-// The largest of 32 lanes' values (a block of 256 values lies in half a wave); a NaN wins.
-__device__ __forceinline__ float max32(float x) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const float y = __shfl_xor(x, o);
-    x = (x > y || x != x) ? x : y;
-  }
-  return x;
+// The largest of 32 lanes' magnitudes (a block of 256 values lies in half a wave), as bits: those
+// of a NaN are above all others.
+__device__ __forceinline__ uint32_t max32(uint32_t x) {
+  x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 15, 15, true));   // lane ^ 1
+  x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 15, 15, true));   // lane ^ 2
+  x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 15, 15, true));  // 7 - lane
+  x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x140, 15, 15, true));  // 15 - lane
+  return max(x, (uint32_t)__shfl_xor((int)x, 16));
 }
 
 // New values x[8] of a block as codes and the block's scale.  A block with a value that is not
 // finite gets a NaN scale: all of its values are then NaN, as they are lost.
-__device__ __forceinline__ float encode(const Book& b, const Border64& exact,
-                                        const double (&x)[8], int (&c)[8]) {
-  float f[8], top = 0.0f;
+template <bool SIGNED>
+__device__ __forceinline__ float encode(const Book& b, const double (&x)[8], int (&c)[8]) {
+  float f[8];
+  uint32_t bits = 0;
 #pragma unroll
   for (int e = 0; e < 8; e++) {
     f[e] = (float)x[e];
-    const float a = fabsf(f[e]);
-    top = (top > a || top != top) ? top : a;
+    bits = max(bits, __builtin_bit_cast(uint32_t, f[e]) & 0x7fffffffu);
   }
-  top = max32(top);
-  if (top == __builtin_inff()) top = __builtin_nanf("");
+  bits = max32(bits);
+  float top = __builtin_bit_cast(float, bits);
+  if (bits >= 0x7f800000u) top = __builtin_nanf("");
   // A scale below fp32's normal range has no fp32 reciprocal: both sides times 2^64 then.
   const bool low = top < 0x1p-100f;
   const float up = low ? 0x1p64f : 1.0f;
   const float inv = top > 0.0f ? __builtin_amdgcn_rcpf(top * up) : 0.0f;
+  if (__any(low)) {  // (rare: kept apart, so that its products are not always paid for)
 #pragma unroll
-  for (int e = 0; e < 8; e++) c[e] = nearest_code(b, exact, x[e], f[e] * up, (double)top, inv);
+    for (int e = 0; e < 8; e++) f[e] *= up;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; e++) c[e] = nearest_code<SIGNED>(b, x[e], f[e], top, inv);
   return top;
 }
 
-template <typename T>
+// FULL: all eight values are in the tensor and its pointers are aligned.
+template <typename T, bool FULL>
 __device__ __forceinline__ void step8(const StepTensor8& t, int64_t i, bool vec,
                                       const StepScalars& s, const Book* books, double b1,
                                       double b2, float eps) {
@@ -428,34 +443,43 @@ __device__ __forceinline__ void step8(const StepTensor8& t, int64_t i, bool vec,
   int cm[8], cv[8];
   T* tp = static_cast<T*>(t.p);
   uint8_t *tm = static_cast<uint8_t*>(t.m), *tv = static_cast<uint8_t*>(t.v);
-  const int64_t blk = i / kStateBlock;
-  const bool live = i < t.n;
-  load8(static_cast<const T*>(t.g), i, t.n, vec, g);
-  load8_codes(tm, i, t.n, vec, cm);
-  load8_codes(tv, i, t.n, vec, cv);
-  load8(tp, i, t.n, vec, p);
-  const bool any = blk * kStateBlock < t.n;
+  const int64_t blk = i / kStateBlock, n = FULL ? i + 8 : t.n;
+  vec |= FULL;
+  load8(static_cast<const T*>(t.g), i, n, vec, g);
+  load8_codes(tm, i, n, vec, cm);
+  load8_codes(tv, i, n, vec, cv);
+  load8(tp, i, n, vec, p);
+  const bool any = FULL || blk * kStateBlock < n;
   const double sm = any ? (double)t.ms[blk] : 0.0, sv = any ? (double)t.vs[blk] : 0.0;
+  const double d1 = 1.0 - b1, d2 = 1.0 - b2;
   double m[8], v[8];
 #pragma unroll
   for (int e = 0; e < 8; e++) {
     const double x = (double)g[e] * s.coef;
-    const bool in = i + e < t.n;
-    m[e] = in ? books[0].value[cm[e]] * sm * b1 + x * (1.0 - b1) : 0.0;
-    v[e] = in ? books[1].value[cv[e]] * sv * b2 + (x * x) * (1.0 - b2) : 0.0;
+    const bool in = FULL || i + e < n;
+    m[e] = in ? books[0].value[cm[e]] * sm * b1 + x * d1 : 0.0;
+    v[e] = in ? books[1].value[cv[e]] * sv * b2 + (x * x) * d2 : 0.0;
     p[e] = p[e] * s.keep - s.size * ratio((float)m[e], (float)v[e], s.root, eps);
   }
-  const float topm = encode(books[0], kBorders[0], m, cm);
-  const float topv = encode(books[1], kBorders[1], v, cv);
-  if (live) {
-    store8(tp, i, t.n, vec, p);
-    store8_codes(tm, i, t.n, vec, cm);
-    store8_codes(tv, i, t.n, vec, cv);
+  const float topm = encode<true>(books[0], m, cm), topv = encode<false>(books[1], v, cv);
+  if (FULL || i < n) {
+    store8(tp, i, n, vec, p);
+    store8_codes(tm, i, n, vec, cm);
+    store8_codes(tv, i, n, vec, cv);
   }
   if (any && (threadIdx.x & 31) == 0) {
     t.ms[blk] = topm;
     t.vs[blk] = topv;
   }
+}
+
+template <typename T>
+__device__ __forceinline__ void step8_of(const StepTensor8& t, int64_t i, bool vec,
+                                         const StepScalars& s, const Book* books, double b1,
+                                         double b2, float eps) {
+  const int64_t end = i - threadIdx.x % 64 * 8 + 512;  // the wave's
+  if (vec && end <= t.n) step8<T, true>(t, i, true, s, books, b1, b2, eps);
+  else step8<T, false>(t, i, vec, s, books, b1, b2, eps);
 }
 
 __device__ __forceinline__ void books_to_lds(Book* books) {
@@ -479,9 +503,9 @@ __global__ __launch_bounds__(256) void k_adamw8(Table<StepTensor8> tab,
     const StepTensor8& t = tab.t[i];
     const bool vec = tab.flags[i] & kVec;
     switch (tab.flags[i] & (kVec - 1)) {
-      case MXS_DTYPE_F16: step8<_Float16>(t, at, vec, s, books, b1, b2, eps); break;
-      case MXS_DTYPE_BF16: step8<__bf16>(t, at, vec, s, books, b1, b2, eps); break;
-      default: step8<float>(t, at, vec, s, books, b1, b2, eps);
+      case MXS_DTYPE_F16: step8_of<_Float16>(t, at, vec, s, books, b1, b2, eps); break;
+      case MXS_DTYPE_BF16: step8_of<__bf16>(t, at, vec, s, books, b1, b2, eps); break;
+      default: step8_of<float>(t, at, vec, s, books, b1, b2, eps);
     }
   }
 }
@@ -618,7 +642,7 @@ int mxs_grad_norm(int count, const void* const* grads, const int64_t* sizes, con
   }
   const int rc = flush();
   if (rc != MXS_OK) return rc;
-  hipLaunchKernelGGL(k_norm_finish, dim3(1), dim3(256), 0, stream, partial, groups, grad_scale,
+  hipLaunchKernelGGL(k_norm_finish, dim3(1), dim3(1024), 0, stream, partial, groups, grad_scale,
                      out);
   return launched();
 }
