@@ -626,7 +626,8 @@ int mxs_grad_norm(int count, const void* const* grads, const int64_t* sizes, con
  * scale * book[code], m over the signed and v over the unsigned 8-bit dynamic map; the new scale
  * is the block's largest magnitude (NaN when a value is not finite) and the new code the nearest
  * one, the lower of two as near, decided in fp64.  No two written tensors may overlap.
- * workspace: 64 bytes, 8-byte aligned. */
+ * workspace: mxs_adamw_workspace_bytes(count, sizes), 8-byte aligned. */
+int64_t mxs_adamw_workspace_bytes(int count, const int64_t* sizes);
 int mxs_adamw_step(int count, void* const* params, const void* const* grads, void* const* avgs,
                    void* const* avg_sqs, float* const* avg_scales, float* const* avg_sq_scales,
                    const int64_t* sizes, const int* dtypes, int state_bits, float* step, double lr,

@@ -111,6 +111,7 @@ _SIGNATURES = {
     "mxs_nf4_linear_bwd_dx_pair_workspace_bytes": [I32, I32, I32, I32],
     "mxs_grad_norm_workspace_bytes": [I32, P],
     "mxs_grad_norm": [I32, P, P, P, P, P, P, P],
+    "mxs_adamw_workspace_bytes": [I32, P],
     "mxs_adamw_step": [I32, P, P, P, P, P, P, P, P, I32, P, F64, P, F64, F64, F64, F64, P, F64, P,
                        P, P, P],
     "mxs_state_values": [P, P, I64, I32, P, P],
@@ -127,6 +128,7 @@ _RESTYPES = {"mxs_nf4_dequant_layer_plan": ctypes.c_int64,
              "mxs_nf4_linear_bwd_dx_sum_workspace_bytes": ctypes.c_int64,
              "mxs_nf4_linear_bwd_dx_pair_workspace_bytes": ctypes.c_int64,
              "mxs_grad_norm_workspace_bytes": ctypes.c_int64,
+             "mxs_adamw_workspace_bytes": ctypes.c_int64,
              "mxs_head_ce_workspace_bytes": ctypes.c_int64}
 
 

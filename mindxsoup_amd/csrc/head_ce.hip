@@ -841,8 +841,8 @@ __global__ __launch_bounds__(kThreads) void k_ce_dh(CeArgs a, int nx, int ny) {
 // dh rows = the shares' sum, with the scales, to their places in [T, D].
 template <typename T, bool SHIFT>
 __global__ __launch_bounds__(256) void k_ce_dh_sum(CeArgs a) {
-  const int n = piece_rows(a), row = (int)blockIdx.y;
-  const int d = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 4;
+  const int n = piece_rows(a), row = (int)blockIdx.x;
+  const int d = ((int)blockIdx.y * 256 + (int)threadIdx.x) * 4;
   if (row >= n || d >= a.D) return;
   float4_t x = {0, 0, 0, 0};
   const float* p = a.part + (int64_t)row * a.D + d;
@@ -1059,7 +1059,7 @@ static CePlan ce_plan(int T, int V, int D, bool grads, int cus) {
   p.vp = (int64_t)((V + kVocabTile - 1) / kVocabTile) * kVocabTile;
   int64_t most = kRowPad;
   if (grads)
-    while (2 * most * p.vp * 2 <= kPieceBytes && most < p.Tp) most *= 2;
+    while (2 * most * p.vp * 2 <= kPieceBytes && most < p.Tp && most < 32768) most *= 2;
   else
     while (most < p.Tp && most < 8192) most *= 2;  // 8 KB of statistics a row at 128 K columns
   p.pieces = (int)((p.Tp + most - 1) / most);
@@ -1210,7 +1210,7 @@ static int run_ce(CeArgs a, const CePlan& p, int cus, hipStream_t stream) {
     }
     if (a.dh) {
       CE_TRY(shift ? (dh_of<T, true>(a, p, stream)) : (dh_of<T, false>(a, p, stream)));
-      const dim3 grid((a.D / 4 + 255) / 256, a.rows);
+      const dim3 grid(a.rows, (a.D / 4 + 255) / 256);
       if (shift)
         hipLaunchKernelGGL((k_ce_dh_sum<T, true>), grid, dim3(256), 0, stream, a);
       else

@@ -2,10 +2,12 @@
 // step over many parameter tensors with its two states in fp32 or in 8 bits.
 //
 // All of it is bound by HBM: every gradient, parameter and state is read once and written once.
-// Tensors travel to a launch in its kernel arguments (pointers and sizes, at most 4 KB, so 86
-// fp32-state or 63 8-bit-state tensors a launch; 228 gradients of a norm), so a step copies
-// nothing to the device and can be captured: a workgroup finds its tensor by a binary search over
-// the first chunk of each.
+// Tensors travel in kernel arguments (4 KB of pointers and sizes at most), so nothing is copied to
+// the device and a call can be captured.  The norm reads them there (228 gradients a launch); the
+// step's first kernels, one for every 99 tensors with fp32 states or 70 with 8-bit ones, write
+// them to a table in the workspace, and one launch then runs over all tensors: with a launch for
+// every 63 tensors the step of 392 adapters with 8-bit states took 138 us, 8 us of each launch its
+// beginning and end.
 //
 // 8-bit states: blocks of 256 values in storage order share one fp32 scale, the largest magnitude;
 // a value is kept as the code of the nearest of 256 book values times that scale.  The update
@@ -21,7 +23,7 @@ typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
 typedef double double2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kStateBlock = 256;  // 8-bit values per scale
-constexpr int kStepArgs = 3900;   // bytes of a launch's tensor table
+constexpr int kTableArgs = 3960;  // bytes of tensors in a launch's arguments
 
 // ---- code books -------------------------------------------------------------------------------
 
@@ -202,30 +204,33 @@ __device__ __forceinline__ void store8_codes(uint8_t* p, int64_t i, int64_t n, b
 
 // ---- tables -----------------------------------------------------------------------------------
 
+// A tensor of a step, or 2^31 values of one: chunks [start, next entry's start).
+constexpr uint32_t kVecBit = 0x80000000u;  // of `start`: the pointers are 16-byte aligned
+
 struct StepTensor {
   void* p;
   const void* g;
   void *m, *v;
-  int64_t n;
+  uint32_t n, start;
 };
-struct StepTensor8 : StepTensor {
+struct StepTensor8 {
+  void* p;
+  const void* g;
+  void *m, *v;
   float *ms, *vs;
+  uint32_t n, start;
 };
 
-// Tensors of one launch; flags: dtype (MXS_DTYPE_*) and kVec.
-constexpr int kVec = 16;
-template <typename T>
-struct Table {
-  static constexpr int N = (kStepArgs - 8) / (sizeof(T) + 5);
-  T t[N];
-  int start[N + 1];  // chunks of tensor i: [start[i], start[i + 1])
-  uint8_t flags[N];
-  int count;
+template <typename E>
+struct StepPart {  // entries of one set-up launch
+  static constexpr int N = kTableArgs / sizeof(E);
+  E t[N];
 };
 
+constexpr int kVec = 16;  // of the norm's flags, beside MXS_DTYPE_*
 // Gradients of one launch of the norm; a longer one than 2^31 values takes several entries.
 struct NormTable {
-  static constexpr int N = (kStepArgs - 8) / 17;
+  static constexpr int N = (kTableArgs - 8) / 17;
   const void* g[N];
   uint32_t n[N];
   int start[N + 1];
@@ -243,6 +248,26 @@ __device__ __forceinline__ int tensor_of(const Tab& tab, int c) {
     else hi = mid;
   }
   return lo;
+}
+
+// The entry of chunk `c` (uniform) of a step's table: halved down to 256 entries, which the lanes
+// look through together.
+template <typename E>
+__device__ __forceinline__ int entry_of(const E* tab, int count, uint32_t c) {
+  int lo = 0, hi = count;
+  while (hi - lo > 256) {
+    const int mid = (lo + hi) >> 1;
+    if (c >= (tab[mid].start & ~kVecBit)) lo = mid;
+    else hi = mid;
+  }
+  int n = 0;
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int i = lo + 64 * j + lane;
+    n += __popcll(__ballot(i < hi && (tab[i < hi ? i : lo].start & ~kVecBit) <= c));
+  }
+  return __builtin_amdgcn_readfirstlane(lo + n - 1);
 }
 
 // ---- gradient norm ----------------------------------------------------------------------------
@@ -319,25 +344,40 @@ struct StepScalars {
   int skip;       // an overflow was found: nothing is changed
 };
 
-__global__ void k_adamw_scalars(StepScalars* out, float* step, double lr, const float* lr_dev,
-                                double beta1, double beta2, double weight_decay,
-                                const float* norm, double max_norm, const float* grad_scale,
-                                const float* found_inf) {
-  const int skip = found_inf && found_inf[0] != 0.0f;
-  const float t = step[0] + 1.0f;
-  if (lr_dev) lr = (double)lr_dev[0];
+struct StepInputs {
+  float* step;
+  double lr;
+  const float* lr_dev;
+  double beta1, beta2, weight_decay;
+  const float* norm;
+  double max_norm;
+  const float *grad_scale, *found_inf;
+};
+
+// Entries of the table from kernel arguments to memory; the first launch of a step also computes
+// what its values share.
+template <typename E>
+__global__ __launch_bounds__(256) void k_adamw_setup(StepPart<E> part, int count, E* table,
+                                                     StepScalars* out, StepInputs in) {
+  const uint32_t* src = reinterpret_cast<const uint32_t*>(part.t);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(table);
+  for (int i = threadIdx.x; i < count * (int)(sizeof(E) / 4); i += 256) dst[i] = src[i];
+  if (!out || threadIdx.x) return;
+  const int skip = in.found_inf && in.found_inf[0] != 0.0f;
+  const float t = in.step[0] + 1.0f;
+  const double lr = in.lr_dev ? (double)in.lr_dev[0] : in.lr;
   double coef = 1.0;
-  if (norm) {
-    coef = max_norm / ((double)norm[0] + 1e-6);
+  if (in.norm) {
+    coef = in.max_norm / ((double)in.norm[0] + 1e-6);
     if (coef > 1.0) coef = 1.0;  // a NaN stays one
   }
-  if (grad_scale) coef /= (double)grad_scale[0];
+  if (in.grad_scale) coef /= (double)in.grad_scale[0];
   out->coef = coef;
-  out->keep = (float)(1.0 - lr * weight_decay);
-  out->size = (float)(lr / (1.0 - pow(beta1, (double)t)));
-  out->root = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t)));
+  out->keep = (float)(1.0 - lr * in.weight_decay);
+  out->size = (float)(lr / (1.0 - pow(in.beta1, (double)t)));
+  out->root = (float)(1.0 / sqrt(1.0 - pow(in.beta2, (double)t)));
   out->skip = skip;
-  if (!skip) step[0] = t;
+  if (!skip) in.step[0] = t;
 }
 
 // m / (sqrt(v) root + eps) with the hardware's root and reciprocal, each within one step of fp32;
@@ -375,23 +415,19 @@ __device__ __forceinline__ void step32(const StepTensor& t, int64_t i, bool vec,
 }
 
 // fp32 states, one pass: 28 bytes a value with fp32 parameters, 22 with 16-bit ones.
-__global__ __launch_bounds__(256) void k_adamw(Table<StepTensor> tab, const StepScalars* scalars,
-                                               float b1, float b2, float c1, float c2,
-                                               float eps) {
+template <typename T>
+__global__ __launch_bounds__(256) void k_adamw(const StepTensor* __restrict__ tab, int count,
+                                               const StepScalars* scalars, float b1, float b2,
+                                               float c1, float c2, float eps) {
   const StepScalars s = *scalars;
   if (s.skip) return;
-  const int c = (int)blockIdx.x, i = tensor_of(tab, c);
-  const int64_t at = (int64_t)(c - tab.start[i]) * kStepChunk + threadIdx.x * 8;
-  const StepTensor& t = tab.t[i];
-  if (at >= t.n) return;
-  const bool vec = tab.flags[i] & kVec;
-  switch (tab.flags[i] & (kVec - 1)) {
-    case MXS_DTYPE_F16: step32<_Float16>(t, at, vec, s, b1, b2, c1, c2, eps); break;
-    case MXS_DTYPE_BF16: step32<__bf16>(t, at, vec, s, b1, b2, c1, c2, eps); break;
-    default: step32<float>(t, at, vec, s, b1, b2, c1, c2, eps);
-  }
+  const StepTensor& t = tab[entry_of(tab, count, blockIdx.x)];
+  const int64_t at =
+      (int64_t)(blockIdx.x - (t.start & ~kVecBit)) * kStepChunk + threadIdx.x * 8;
+  if (at < t.n) step32<T>(t, at, (t.start & kVecBit) != 0, s, b1, b2, c1, c2, eps);
 }
 
+constexpr uint32_t kStep8Groups = 2048;  // workgroups at most (1024 and 4096: within 1 %, 2 % more)
 constexpr int kStep8Chunk = 2048;  // values of a workgroup, 8-bit states: 8 blocks
 
 // The largest of 32 lanes' magnitudes (a block of 256 values lies in half a wave), as bits: those
@@ -431,55 +467,48 @@ __device__ __forceinline__ float encode(const Book& b, const double (&x)[8], int
   return top;
 }
 
-// FULL: all eight values are in the tensor and its pointers are aligned.
-template <typename T, bool FULL>
-__device__ __forceinline__ void step8(const StepTensor8& t, int64_t i, bool vec,
+// Eight values of a step as they are loaded.
+template <typename T>
+struct Raw8 {
+  static constexpr int W = sizeof(T) / 2;
+  u32x4 p[W], g[W];
+  u32x2 m, v;
+  float sm, sv;
+};
+
+template <typename T>
+__device__ __forceinline__ void widen(const u32x4 (&x)[sizeof(T) / 2], float (&f)[8]) {
+  typedef T vec_t __attribute__((ext_vector_type(16 / sizeof(T))));
+  constexpr int W = 16 / sizeof(T);
+#pragma unroll
+  for (int q = 0; q < 8 / W; q++) {
+    const vec_t v = __builtin_bit_cast(vec_t, x[q]);
+#pragma unroll
+    for (int e = 0; e < W; e++) f[q * W + e] = (float)v[e];
+  }
+}
+
+// The step of eight values; `in` says which of them exist (ALL: every one).
+template <bool ALL>
+__device__ __forceinline__ void step8(float (&p)[8], const float (&g)[8], int (&cm)[8],
+                                      int (&cv)[8], float& sm, float& sv, int in,
                                       const StepScalars& s, const Book* books, double b1,
                                       double b2, float eps) {
   // Products and sums rounded one by one: (9 x + y) / 10 of numbers as short as these can lie
   // half way between two fp32 scales, where a fused sum would decide otherwise than the formula.
 #pragma clang fp contract(off)
-  float p[8], g[8];
-  int cm[8], cv[8];
-  T* tp = static_cast<T*>(t.p);
-  uint8_t *tm = static_cast<uint8_t*>(t.m), *tv = static_cast<uint8_t*>(t.v);
-  const int64_t blk = i / kStateBlock, n = FULL ? i + 8 : t.n;
-  vec |= FULL;
-  load8(static_cast<const T*>(t.g), i, n, vec, g);
-  load8_codes(tm, i, n, vec, cm);
-  load8_codes(tv, i, n, vec, cv);
-  load8(tp, i, n, vec, p);
-  const bool any = FULL || blk * kStateBlock < n;
-  const double sm = any ? (double)t.ms[blk] : 0.0, sv = any ? (double)t.vs[blk] : 0.0;
-  const double d1 = 1.0 - b1, d2 = 1.0 - b2;
+  const double d1 = 1.0 - b1, d2 = 1.0 - b2, sm64 = (double)sm, sv64 = (double)sv;
   double m[8], v[8];
 #pragma unroll
   for (int e = 0; e < 8; e++) {
     const double x = (double)g[e] * s.coef;
-    const bool in = FULL || i + e < n;
-    m[e] = in ? books[0].value[cm[e]] * sm * b1 + x * d1 : 0.0;
-    v[e] = in ? books[1].value[cv[e]] * sv * b2 + (x * x) * d2 : 0.0;
+    const bool live = ALL || e < in;
+    m[e] = live ? books[0].value[cm[e]] * sm64 * b1 + x * d1 : 0.0;
+    v[e] = live ? books[1].value[cv[e]] * sv64 * b2 + (x * x) * d2 : 0.0;
     p[e] = p[e] * s.keep - s.size * ratio((float)m[e], (float)v[e], s.root, eps);
   }
-  const float topm = encode<true>(books[0], m, cm), topv = encode<false>(books[1], v, cv);
-  if (FULL || i < n) {
-    store8(tp, i, n, vec, p);
-    store8_codes(tm, i, n, vec, cm);
-    store8_codes(tv, i, n, vec, cv);
-  }
-  if (any && (threadIdx.x & 31) == 0) {
-    t.ms[blk] = topm;
-    t.vs[blk] = topv;
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void step8_of(const StepTensor8& t, int64_t i, bool vec,
-                                         const StepScalars& s, const Book* books, double b1,
-                                         double b2, float eps) {
-  const int64_t end = i - threadIdx.x % 64 * 8 + 512;  // the wave's
-  if (vec && end <= t.n) step8<T, true>(t, i, true, s, books, b1, b2, eps);
-  else step8<T, false>(t, i, vec, s, books, b1, b2, eps);
+  sm = encode<true>(books[0], m, cm);
+  sv = encode<false>(books[1], v, cv);
 }
 
 __device__ __forceinline__ void books_to_lds(Book* books) {
@@ -489,24 +518,88 @@ __device__ __forceinline__ void books_to_lds(Book* books) {
   __syncthreads();
 }
 
-// 8-bit states, one pass: 10 bytes a value with 16-bit parameters, 16 with fp32 ones.
-__global__ __launch_bounds__(256) void k_adamw8(Table<StepTensor8> tab,
+// 8-bit states, one pass: 10 bytes a value with 16-bit parameters, 16 with fp32 ones.  A wave takes
+// 512 values, two blocks.  About 70 vector instructions a value fill the pass as much as its bytes
+// do: 323 M bf16 values take 959 us, 3.4 TB/s.  Loading ahead of the values in hand cost more
+// registers, and so waves, than it gained (1121 us); the entry read anew for every chunk, behind
+// stores that might have changed it, 1130 us.
+template <typename T>
+__global__ __launch_bounds__(256, 4) void k_adamw8(const StepTensor8* __restrict__ tab, int count,
+                                                   uint32_t chunks,
                                                 const StepScalars* scalars, double b1, double b2,
                                                 float eps) {
   __shared__ Book books[2];
   const StepScalars s = *scalars;
   if (s.skip) return;
-  books_to_lds(books);
-  for (int c = (int)blockIdx.x; c < tab.start[tab.count]; c += (int)gridDim.x) {
-    const int i = tensor_of(tab, c);
-    const int64_t at = (int64_t)(c - tab.start[i]) * kStep8Chunk + threadIdx.x * 8;
-    const StepTensor8& t = tab.t[i];
-    const bool vec = tab.flags[i] & kVec;
-    switch (tab.flags[i] & (kVec - 1)) {
-      case MXS_DTYPE_F16: step8_of<_Float16>(t, at, vec, s, books, b1, b2, eps); break;
-      case MXS_DTYPE_BF16: step8_of<__bf16>(t, at, vec, s, books, b1, b2, eps); break;
-      default: step8_of<float>(t, at, vec, s, books, b1, b2, eps);
+  uint32_t start = 0, end = 0;  // chunks of the entry in hand; most steps to the next stay in it
+  StepTensor8 t = {};
+  int64_t at = 0;      // the lane's first value
+  bool whole = false;  // the wave's 512 values exist and are aligned
+  auto place = [&](uint32_t c) {
+    if (c >= end) {
+      const int i = entry_of(tab, count, c);
+      t = tab[i];
+      start = t.start & ~kVecBit;
+      end = i + 1 < count ? tab[i + 1].start & ~kVecBit : chunks;
     }
+    at = (int64_t)(c - start) * kStep8Chunk + threadIdx.x * 8;
+    whole = (t.start & kVecBit) && at - threadIdx.x % 64 * 8 + 512 <= t.n;
+  };
+  auto load = [&](Raw8<T>& r) {
+    if (!whole) return;
+    const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const T*>(t.p) + at);
+    const u32x4* g = reinterpret_cast<const u32x4*>(static_cast<const T*>(t.g) + at);
+#pragma unroll
+    for (int q = 0; q < Raw8<T>::W; q++) r.g[q] = g[q], r.p[q] = p[q];
+    r.m = *reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(t.m) + at);
+    r.v = *reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(t.v) + at);
+    r.sm = t.ms[at / kStateBlock];
+    r.sv = t.vs[at / kStateBlock];
+  };
+  Raw8<T> raw;
+  place(blockIdx.x);
+  load(raw);  // on its way while the books come
+  books_to_lds(books);
+  for (uint32_t c = blockIdx.x;;) {
+    T* tp = static_cast<T*>(t.p);
+    uint8_t *tm = static_cast<uint8_t*>(t.m), *tv = static_cast<uint8_t*>(t.v);
+    const int64_t i = at, n = t.n, blk = i / kStateBlock;
+    float p[8], g[8], sm, sv;
+    int cm[8], cv[8];
+    if (whole) {
+      widen<T>(raw.p, p);
+      widen<T>(raw.g, g);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        cm[e] = (raw.m[e >> 2] >> (8 * (e & 3))) & 255;
+        cv[e] = (raw.v[e >> 2] >> (8 * (e & 3))) & 255;
+      }
+      sm = raw.sm, sv = raw.sv;
+      step8<true>(p, g, cm, cv, sm, sv, 8, s, books, b1, b2, eps);
+      store8(tp, i, i + 8, true, p);
+      store8_codes(tm, i, i + 8, true, cm);
+      store8_codes(tv, i, i + 8, true, cv);
+    } else {
+      const bool any = blk * kStateBlock < n;
+      load8(static_cast<const T*>(t.g), i, n, false, g);
+      load8_codes(tm, i, n, false, cm);
+      load8_codes(tv, i, n, false, cv);
+      load8(tp, i, n, false, p);
+      sm = any ? t.ms[blk] : 0.0f, sv = any ? t.vs[blk] : 0.0f;
+      const int in = (int)(n - i < 0 ? 0 : n - i < 8 ? n - i : 8);
+      step8<false>(p, g, cm, cv, sm, sv, in, s, books, b1, b2, eps);
+      store8(tp, i, n, false, p);
+      store8_codes(tm, i, n, false, cm);
+      store8_codes(tv, i, n, false, cv);
+    }
+    if ((threadIdx.x & 31) == 0 && blk * kStateBlock < n) {
+      t.ms[blk] = sm;
+      t.vs[blk] = sv;
+    }
+    c += gridDim.x;
+    if (c >= chunks) break;
+    place(c);
+    load(raw);
   }
 }
 
@@ -551,35 +644,57 @@ static bool dtype_ok(int d) {
   return d == MXS_DTYPE_F16 || d == MXS_DTYPE_F32 || d == MXS_DTYPE_BF16;
 }
 
-// Puts one tensor after the other into a table and calls launch(table, chunks, chunks before it)
-// whenever it is full or holds 2^30 chunks' worth, and at the end.
-template <typename T, typename Fill, typename Launch>
-static int tables(int count, const int64_t* sizes, int64_t chunk, Fill fill, Launch launch) {
-  Table<T> tab;
-  tab.count = 0;
-  tab.start[0] = 0;
-  int64_t before = 0;
-  for (int i = 0; i <= count; i++) {
-    const int64_t chunks = i < count ? (sizes[i] + chunk - 1) / chunk : 0;
-    const bool full = tab.count == Table<T>::N || tab.start[tab.count] + chunks > (1 << 30);
-    if (tab.count && (i == count || full)) {
-      const int rc = launch(tab, tab.start[tab.count], before);
-      if (rc != MXS_OK) return rc;
-      before += tab.start[tab.count];
-      tab.count = 0;
-    }
-    if (chunks > (1 << 30)) return MXS_ERR_SIZE;
-    if (i == count || chunks == 0) continue;
-    fill(tab.t[tab.count], tab.flags[tab.count], i);
-    tab.start[tab.count + 1] = tab.start[tab.count] + (int)chunks;
-    tab.count++;
-  }
-  return MXS_OK;
-}
-
 static int launched() {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? MXS_OK : (int)e;
+}
+
+// One step over tensors whose parameters are T: the table's entries, then the launch over them.
+// `table` has room for the entries; main(table, entries, chunks) launches.
+constexpr int64_t kEntryValues = (int64_t)1 << 31;  // of one entry
+
+static int64_t step_entries(int count, const int64_t* sizes) {
+  int64_t n = 0;
+  for (int i = 0; i < count; i++) n += (sizes[i] + kEntryValues - 1) / kEntryValues;
+  return n;
+}
+
+template <typename E, typename Fill, typename Main>
+static int run_step(int count, const int64_t* sizes, const int* dtypes, int dtype, int64_t chunk,
+                    E* table, StepScalars* scalars, bool& first, const StepInputs& in,
+                    hipStream_t stream, Fill fill, Main main) {
+  StepPart<E> part;
+  int held = 0, entries = 0;
+  int64_t chunks = 0;
+  auto flush = [&]() {
+    if (held == 0) return MXS_OK;
+    hipLaunchKernelGGL(k_adamw_setup<E>, dim3(1), dim3(256), 0, stream, part, held,
+                       table + entries, first ? scalars : nullptr, in);
+    first = false;
+    entries += held;
+    held = 0;
+    return launched();
+  };
+  for (int i = 0; i < count; i++) {
+    if (dtypes[i] != dtype) continue;
+    for (int64_t at = 0; at < sizes[i]; at += kEntryValues) {
+      const int64_t n = sizes[i] - at < kEntryValues ? sizes[i] - at : kEntryValues;
+      if (held == StepPart<E>::N) {
+        const int rc = flush();
+        if (rc != MXS_OK) return rc;
+      }
+      const bool vec = fill(part.t[held], i, at);
+      part.t[held].n = (uint32_t)n;
+      part.t[held].start = (uint32_t)chunks | (vec ? kVecBit : 0u);
+      chunks += (n + chunk - 1) / chunk;
+      if (chunks >= 1 << 24) return MXS_ERR_SIZE;  // a launch has fewer than 2^32 lanes
+      held++;
+    }
+  }
+  const int rc = flush();
+  if (rc != MXS_OK || entries == 0) return rc;
+  main(table, entries, (uint32_t)chunks);
+  return launched();
 }
 
 static int64_t norm_chunks(int count, const int64_t* sizes) {
@@ -647,6 +762,13 @@ int mxs_grad_norm(int count, const void* const* grads, const int64_t* sizes, con
   return launched();
 }
 
+int64_t mxs_adamw_workspace_bytes(int count, const int64_t* sizes) {
+  if (count < 0 || (count && !sizes)) return MXS_ERR_ARG;
+  for (int i = 0; i < count; i++)
+    if (sizes[i] < 0) return MXS_ERR_ARG;
+  return 64 + (int64_t)sizeof(StepTensor8) * step_entries(count, sizes);
+}
+
 int mxs_adamw_step(int count, void* const* params, const void* const* grads, void* const* avgs,
                    void* const* avg_sqs, float* const* avg_scales, float* const* avg_sq_scales,
                    const int64_t* sizes, const int* dtypes, int state_bits, float* step, double lr,
@@ -666,41 +788,54 @@ int mxs_adamw_step(int count, void* const* params, const void* const* grads, voi
     if (sizes[i] && (!params[i] || !grads[i] || !avgs[i] || !avg_sqs[i])) return MXS_ERR_ARG;
     if (sizes[i] && bits8 && (!avg_scales[i] || !avg_sq_scales[i])) return MXS_ERR_ARG;
   }
+  if (step_entries(count, sizes) > (1 << 30)) return MXS_ERR_SIZE;
   StepScalars* scalars = static_cast<StepScalars*>(workspace);
-  hipLaunchKernelGGL(k_adamw_scalars, dim3(1), dim3(1), 0, stream, scalars, step, lr, lr_dev,
-                     beta1, beta2, weight_decay, norm, max_norm, grad_scale, found_inf);
-  int rc = launched();
-  if (rc != MXS_OK) return rc;
-  auto flags_of = [&](int i) {
-    const bool vec = on16(params[i]) && on16(grads[i]) && on16(avgs[i]) && on16(avg_sqs[i]);
-    return (uint8_t)(dtypes[i] | (vec ? kVec : 0));
+  char* table = static_cast<char*>(workspace) + 64;
+  const StepInputs in = {step, lr, lr_dev, beta1, beta2, weight_decay, norm, max_norm, grad_scale,
+                         found_inf};
+  bool first = true;
+  auto base = [&](auto& t, int i, int64_t at) {
+    const int64_t wide = dtypes[i] == MXS_DTYPE_F32 ? 4 : 2, state = bits8 ? 1 : 4;
+    t.p = static_cast<char*>(params[i]) + at * wide;
+    t.g = static_cast<const char*>(grads[i]) + at * wide;
+    t.m = static_cast<char*>(avgs[i]) + at * state;
+    t.v = static_cast<char*>(avg_sqs[i]) + at * state;
+    return on16(t.p) && on16(t.g) && on16(t.m) && on16(t.v);
   };
-  if (!bits8)
-    return tables<StepTensor>(
-        count, sizes, kStepChunk,
-        [&](StepTensor& t, uint8_t& flags, int i) {
-          t = {params[i], grads[i], avgs[i], avg_sqs[i], sizes[i]};
-          flags = flags_of(i);
+  auto of_dtype = [&](auto zero, int dtype) {
+    using T = decltype(zero);
+    if (!bits8)
+      return run_step(
+          count, sizes, dtypes, dtype, kStepChunk, reinterpret_cast<StepTensor*>(table), scalars,
+          first, in, stream, base, [&](const StepTensor* tab, int n, uint32_t chunks) {
+            hipLaunchKernelGGL(k_adamw<T>, dim3(chunks), dim3(256), 0, stream, tab, n, scalars,
+                               (float)beta1, (float)beta2, (float)(1.0 - beta1),
+                               (float)(1.0 - beta2), (float)eps);
+          });
+    return run_step(
+        count, sizes, dtypes, dtype, kStep8Chunk, reinterpret_cast<StepTensor8*>(table), scalars,
+        first, in, stream,
+        [&](StepTensor8& t, int i, int64_t at) {
+          t.ms = avg_scales[i] + at / kStateBlock;
+          t.vs = avg_sq_scales[i] + at / kStateBlock;
+          return base(t, i, at);
         },
-        [&](const Table<StepTensor>& tab, int chunks, int64_t) {
-          hipLaunchKernelGGL(k_adamw, dim3(chunks), dim3(256), 0, stream, tab, scalars,
-                             (float)beta1, (float)beta2, (float)(1.0 - beta1),
-                             (float)(1.0 - beta2), (float)eps);
-          return launched();
+        [&](const StepTensor8* tab, int n, uint32_t chunks) {
+          hipLaunchKernelGGL(k_adamw8<T>, dim3(chunks < kStep8Groups ? chunks : kStep8Groups), dim3(256), 0,
+                             stream, tab, n, chunks, scalars, beta1, beta2, (float)eps);
         });
-  return tables<StepTensor8>(
-      count, sizes, kStep8Chunk,
-      [&](StepTensor8& t, uint8_t& flags, int i) {
-        t.p = params[i], t.g = grads[i], t.m = avgs[i], t.v = avg_sqs[i], t.n = sizes[i];
-        t.ms = avg_scales[i], t.vs = avg_sq_scales[i];
-        flags = flags_of(i);
-      },
-      [&](const Table<StepTensor8>& tab, int chunks, int64_t) {
-        const int grid = chunks < 2048 ? chunks : 2048;
-        hipLaunchKernelGGL(k_adamw8, dim3(grid), dim3(256), 0, stream, tab, scalars, beta1, beta2,
-                           (float)eps);
-        return launched();
-      });
+  };
+  // tensors of one type after the other, over the same table: launches run in order
+  int rc = of_dtype(0.0f, MXS_DTYPE_F32);
+  if (rc == MXS_OK) rc = of_dtype((_Float16)0, MXS_DTYPE_F16);
+  if (rc == MXS_OK) rc = of_dtype((__bf16)0, MXS_DTYPE_BF16);
+  if (rc == MXS_OK && first) {  // no values at all: only the step counts
+    hipLaunchKernelGGL(k_adamw_setup<StepTensor>, dim3(1), dim3(256), 0, stream,
+                       StepPart<StepTensor>{}, 0, reinterpret_cast<StepTensor*>(table), scalars,
+                       in);
+    rc = launched();
+  }
+  return rc;
 }
 
 int mxs_state_values(const void* codes, const float* scale, int64_t n, int is_signed, float* out,
@@ -709,8 +844,8 @@ int mxs_state_values(const void* codes, const float* scale, int64_t n, int is_si
   if (n == 0) return MXS_OK;
   if (!codes || !scale || !out) return MXS_ERR_ARG;
   const int vec = (uintptr_t)codes % 4 == 0 && on16(out);
-  for (int64_t at = 0; at < n; at += (int64_t)1 << 40) {  // a grid's 32 bits of workgroups
-    const int64_t some = n - at < ((int64_t)1 << 40) ? n - at : (int64_t)1 << 40;
+  for (int64_t at = 0; at < n; at += (int64_t)1 << 34) {  // a launch has fewer than 2^32 lanes
+    const int64_t some = n - at < ((int64_t)1 << 34) ? n - at : (int64_t)1 << 34;
     hipLaunchKernelGGL(k_state_values, dim3((unsigned)((some + 4095) / 4096)), dim3(256), 0,
                        stream, static_cast<const uint8_t*>(codes) + at, scale + at / kStateBlock,
                        out + at, some, is_signed ? 0 : 1, vec);

@@ -1674,7 +1674,8 @@ void adamw_step_cuda(TensorList params, TensorList grads, TensorList avgs, Tenso
     TORCH_CHECK(written[i - 1].second <= written[i].first,
                 "two of the tensors that the step writes overlap");
   const int count = as_int((int64_t)n, "the number of parameters");
-  Tensor ws = at::empty({64}, step.options().dtype(at::kByte));
+  Tensor ws = at::empty({mxs_adamw_workspace_bytes(count, sizes.data())},
+                        step.options().dtype(at::kByte));
   ok(mxs_adamw_step(count, p.data(), g.data(), m.data(), v.data(), ms.data(), vs.data(),
                     sizes.data(), dtypes.data(), bits8 ? 8 : 32, step.data_ptr<float>(), lr,
                     scalar_ptr(lr_dev, dev, "lr"), beta1, beta2, eps, weight_decay,
