@@ -18,11 +18,13 @@
 //   lora_bwd_group    lora_bwd for them, small launches shared
 //   mlp_fwd, mlp_bwd  the SwiGLU MLP block of three such projections (solution/mlp.py:33-44)
 //   grad_norm, adamw_step, state_values  the end of a training step over lists of tensors
+//   head_ce, head_ce_grad  the head's cross entropy and its gradients (solution/fused_ce.py:95-148)
 // Autograd ops (one node per call; backward in C++), named as the package's Python Functions
 // they stand for (a node's name() says which ran):
 //   linear         NF4LinearFunction
 //   lora_linear    NF4LoraFunction
 //   lora_siblings  NF4LoraSiblingsFunction
+//   head_cross_entropy  FusedHeadCE
 //
 // Every result is produced by the same kernels, in the same order, as the package's Python
 // path over ctypes, so the two give the same bits.
@@ -1717,6 +1719,177 @@ Tensor state_values_cuda(const Tensor& codes, const Tensor& scale, bool is_signe
   return out;
 }
 
+// ---- the head's cross entropy -----------------------------------------------------------------
+
+// t [rows, cols] with its columns side by side, and its row stride.
+std::pair<Tensor, int64_t> strided_rows(const Tensor& t) {
+  const int64_t cols = t.size(1);
+  if (t.size(0) <= 1) return {t.contiguous(), cols};
+  const Tensor c = t.stride(1) == 1 && t.stride(0) >= cols ? t : t.contiguous();
+  return {c, c.stride(0)};
+}
+
+void head_ce_check(const Tensor& h, const Tensor& w, const Tensor& labels, int64_t reduction) {
+  for (const auto& x : {std::make_pair("hidden", &h), std::make_pair("weight", &w),
+                        std::make_pair("labels", &labels)}) {
+    TORCH_CHECK_VALUE(x.second->is_cuda() || x.second->is_meta(), x.first,
+                      " must be a GPU tensor, found ", x.second->device());
+    TORCH_CHECK_VALUE(x.second->device() == h.device(), x.first, " is on ", x.second->device(),
+                      ", hidden on ", h.device());
+  }
+  TORCH_CHECK_VALUE(w.dim() == 2 && h.dim() >= 1 && h.size(-1) == w.size(1),
+                    "hidden [..., D] and weight [V, D], got ", h.sizes(), " and ", w.sizes());
+  TORCH_CHECK_VALUE(labels.sizes() == h.sizes().slice(0, h.dim() - 1), "labels ", labels.sizes(),
+                    " for hidden ", h.sizes());
+  TORCH_CHECK_VALUE(at::isIntegralType(labels.scalar_type(), false),
+                    "labels must be integers, got ", labels.scalar_type());
+  TORCH_CHECK_VALUE(w.size(0) > 0 && w.size(1) > 0 && w.size(1) % 64 == 0,
+                    "the table is [V >= 1, a multiple of 64], got ", w.sizes());
+  TORCH_CHECK_VALUE(h.scalar_type() == w.scalar_type() &&
+                        (h.scalar_type() == at::kHalf || h.scalar_type() == at::kBFloat16),
+                    "hidden and weight must both be fp16 or both bf16, got ", h.scalar_type(),
+                    " and ", w.scalar_type());
+  TORCH_CHECK_VALUE(reduction >= 0 && reduction <= 2, "reduction ", reduction);
+}
+
+using HeadCe = std::tuple<Tensor, Tensor, Tensor>;
+
+HeadCe head_ce_meta(const Tensor& h, const Tensor& w, const Tensor& labels, int64_t,
+                    int64_t reduction, const OptTensor& row_grad, bool want_loss, bool want_dh,
+                    bool want_dw) {
+  head_ce_check(h, w, labels, reduction);
+  TORCH_CHECK(h.dim() == 2, "hidden must be [T, D], got ", h.sizes());
+  if (row_grad.has_value() && row_grad->defined())
+    TORCH_CHECK(row_grad->scalar_type() == at::kFloat && row_grad->dim() == 1 &&
+                    row_grad->size(0) == h.size(0) && row_grad->device() == h.device(),
+                "row_grad must be fp32 [", h.size(0), "], got ", row_grad->sizes());
+  const auto f32 = h.options().dtype(at::kFloat);
+  Tensor loss, dh, dw;
+  if (want_loss) loss = reduction == 0 ? at::empty({h.size(0)}, f32) : at::empty({}, f32);
+  if (want_dh) dh = at::empty(h.sizes(), f32);
+  if (want_dw) dw = at::empty(w.sizes(), f32);
+  return {loss, dh, dw};
+}
+
+HeadCe head_ce_cuda(const Tensor& h, const Tensor& w, const Tensor& labels, int64_t ignore_index,
+                    int64_t reduction, const OptTensor& row_grad, bool want_loss, bool want_dh,
+                    bool want_dw) {
+  const at::OptionalDeviceGuard guard(h.device());
+  auto out = head_ce_meta(h, w, labels, ignore_index, reduction, row_grad, want_loss, want_dh,
+                          want_dw);
+  const int T = as_int(h.size(0), "T"), D = as_int(h.size(1), "D"), V = as_int(w.size(0), "V");
+  const auto [hr, ldh] = strided_rows(h);
+  auto [wr, ldw] = strided_rows(w);
+  if (ldw % 8 || reinterpret_cast<uintptr_t>(wr.data_ptr()) % 16) {
+    wr = wr.clone(at::MemoryFormat::Contiguous);
+    ldw = D;
+  }
+  const Tensor y = labels.to(at::kLong).contiguous();
+  const Tensor g = row_grad.has_value() && row_grad->defined() ? row_grad->contiguous() : Tensor();
+  const int64_t bytes = mxs_head_ce_workspace_bytes(T, V, D, want_dh, want_dw);
+  TORCH_CHECK(bytes >= 0, "hidden ", h.sizes(), " and weight ", w.sizes(), ": ",
+              why(static_cast<int>(bytes)));
+  Tensor ws = at::empty({bytes}, h.options().dtype(at::kByte));
+  ok(mxs_head_ce(hr.data_ptr(), ldh, wr.data_ptr(), ldw, y.data_ptr<int64_t>(), T, V, D,
+                 float_dtype(h, "hidden"), ignore_index, static_cast<int>(reduction),
+                 ptr<float>(g), ptr<float>(std::get<0>(out)), ptr<float>(std::get<1>(out)),
+                 ptr<float>(std::get<2>(out)), ws.data_ptr(), stream_of(h)),
+     "mxs_head_ce");
+  return out;
+}
+
+Tensor head_ce_grad_meta(const Tensor& unit, const Tensor& g, at::ScalarType dtype) {
+  TORCH_CHECK(unit.scalar_type() == at::kFloat && unit.dim() == 2 && unit.is_contiguous() &&
+                  g.scalar_type() == at::kFloat && g.device() == unit.device() &&
+                  (g.dim() == 0 || (g.dim() == 1 && g.size(0) == unit.size(0))),
+              "unit must be fp32 [rows, cols] and g fp32 [] or [rows], got ", unit.sizes(),
+              " and ", g.sizes());
+  return at::empty(unit.sizes(), unit.options().dtype(dtype));
+}
+
+Tensor head_ce_grad_cuda(const Tensor& unit, const Tensor& g, at::ScalarType dtype) {
+  const at::OptionalDeviceGuard guard(unit.device());
+  Tensor out = head_ce_grad_meta(unit, g, dtype);
+  const Tensor f = g.contiguous();
+  ok(mxs_head_ce_grad(unit.data_ptr<float>(), f.data_ptr<float>(), g.dim() > 0, unit.size(0),
+                      as_int(unit.size(1), "D"), float_dtype(out, "the gradient"), out.data_ptr(),
+                      stream_of(unit)),
+     "mxs_head_ce_grad");
+  return out;
+}
+
+using HeadCeSig = HeadCe(const Tensor&, const Tensor&, const Tensor&, int64_t, int64_t,
+                         const OptTensor&, bool, bool, bool);
+
+// Head and cross entropy (FusedHeadCE of the Python package).  Gradients are computed with the
+// losses and only multiplied in the backward; per-row losses of a trained table are the
+// exception (`again`): their table's gradient needs the factors from above, row by row.
+struct FusedHeadCE : public torch::autograd::Function<FusedHeadCE> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight,
+                        const Tensor& labels, int64_t ignore_index, int64_t reduction,
+                        bool want_dh, bool want_dw) {
+    static auto run = op<HeadCeSig>("mxs_nf4::head_ce");
+    at::AutoDispatchBelowADInplaceOrView below;
+    const bool again = want_dw && reduction == 0;
+    const Tensor h = rows2d(hidden), y = labels.reshape({-1});
+    Tensor loss, dh, dw;
+    std::tie(loss, dh, dw) = run.call(h, weight, y, ignore_index, reduction, std::nullopt, true,
+                                      want_dh && !again, want_dw && !again);
+    ctx->saved_data["again"] = again;
+    ctx->saved_data["ignore"] = ignore_index;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["shape"] = hidden.sizes().vec();
+    ctx->saved_data["dtype"] = hidden.scalar_type();
+    if (again) ctx->save_for_backward({hidden, weight, labels});
+    else ctx->save_for_backward({dh, dw});
+    return reduction == 0 ? loss.view(labels.sizes()) : loss;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    static auto run = op<HeadCeSig>("mxs_nf4::head_ce");
+    static auto scale =
+        op<Tensor(const Tensor&, const Tensor&, at::ScalarType)>("mxs_nf4::head_ce_grad");
+    TORCH_CHECK(!at::GradMode::is_enabled(), "head_cross_entropy has no second derivative");
+    const auto saved = ctx->get_saved_variables();
+    const bool wh = ctx->needs_input_grad(0), ww = ctx->needs_input_grad(1);
+    const auto dtype = ctx->saved_data["dtype"].toScalarType();
+    const int64_t reduction = ctx->saved_data["reduction"].toInt();
+    at::AutoDispatchBelowADInplaceOrView below;
+    Tensor g = grads[0].to(at::kFloat), dh, dw;
+    if (reduction == 0) g = g.reshape({-1}).contiguous();
+    if (ctx->saved_data["again"].toBool()) {
+      std::tie(std::ignore, dh, dw) =
+          run.call(rows2d(saved[0]), saved[1], saved[2].reshape({-1}),
+                   ctx->saved_data["ignore"].toInt(), reduction, g, false, wh, ww);
+      if (dh.defined()) dh = dh.to(dtype);
+      if (dw.defined()) dw = dw.to(dtype);
+    } else {
+      if (wh) dh = scale.call(saved[0], g, dtype);
+      if (ww) dw = scale.call(saved[1], g, dtype);
+    }
+    if (dh.defined()) dh = dh.view(ctx->saved_data["shape"].toIntVector());
+    return {dh, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor head_cross_entropy_autograd(const Tensor& hidden, const Tensor& weight,
+                                   const Tensor& labels, int64_t ignore_index,
+                                   int64_t reduction) {
+  head_ce_check(hidden, weight, labels, reduction);
+  const bool on = at::GradMode::is_enabled();
+  return FusedHeadCE::apply(hidden, weight, labels, ignore_index, reduction,
+                            on && hidden.requires_grad(), on && weight.requires_grad());
+}
+
+Tensor head_cross_entropy_plain(const Tensor& hidden, const Tensor& weight, const Tensor& labels,
+                                int64_t ignore_index, int64_t reduction) {
+  static auto run = op<HeadCeSig>("mxs_nf4::head_ce");
+  head_ce_check(hidden, weight, labels, reduction);
+  Tensor loss = std::get<0>(run.call(rows2d(hidden), weight, labels.reshape({-1}), ignore_index,
+                                     reduction, std::nullopt, true, false, false));
+  return reduction == 0 ? loss.view(labels.sizes()) : loss;
+}
+
 }  // namespace
 
 namespace mxs_lists {
@@ -1780,6 +1953,12 @@ TORCH_LIBRARY(mxs_nf4, m) {
         "float weight_decay, Tensor? norm, float max_norm, Tensor? grad_scale, "
         "Tensor? found_inf) -> ()");
   m.def("state_values(Tensor codes, Tensor scale, bool signed) -> Tensor");
+  m.def("head_ce(Tensor hidden, Tensor weight, Tensor labels, int ignore_index, int reduction, "
+        "Tensor? row_grad, bool want_loss, bool want_dh, bool want_dw) "
+        "-> (Tensor, Tensor, Tensor)");
+  m.def("head_ce_grad(Tensor unit, Tensor g, ScalarType dtype) -> Tensor");
+  m.def("head_cross_entropy(Tensor hidden, Tensor weight, Tensor labels, int ignore_index, "
+        "int reduction) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(mxs_nf4, CUDA, m) {
@@ -1795,6 +1974,8 @@ TORCH_LIBRARY_IMPL(mxs_nf4, CUDA, m) {
   m.impl("grad_norm", &grad_norm_cuda);
   m.impl("adamw_step", &adamw_step_cuda);
   m.impl("state_values", &state_values_cuda);
+  m.impl("head_ce", &head_ce_cuda);
+  m.impl("head_ce_grad", &head_ce_grad_cuda);
 }
 
 TORCH_LIBRARY_IMPL(mxs_nf4, Meta, m) {
@@ -1810,6 +1991,8 @@ TORCH_LIBRARY_IMPL(mxs_nf4, Meta, m) {
   m.impl("grad_norm", &grad_norm_meta);
   m.impl("adamw_step", &adamw_step_meta);
   m.impl("state_values", &state_values_meta);
+  m.impl("head_ce", &head_ce_meta);
+  m.impl("head_ce_grad", &head_ce_grad_meta);
 }
 
 // The autograd ops: the same node with or without grad mode (without it, or with no input
@@ -1818,10 +2001,12 @@ TORCH_LIBRARY_IMPL(mxs_nf4, Autograd, m) {
   m.impl("linear", &linear_autograd);
   m.impl("lora_linear", &lora_linear_autograd);
   m.impl("lora_siblings", &lora_siblings_autograd);
+  m.impl("head_cross_entropy", &head_cross_entropy_autograd);
 }
 
 TORCH_LIBRARY_IMPL(mxs_nf4, CompositeExplicitAutograd, m) {
   m.impl("linear", &linear_plain);
   m.impl("lora_linear", &lora_linear_plain);
   m.impl("lora_siblings", &lora_siblings_plain);
+  m.impl("head_cross_entropy", &head_cross_entropy_plain);
 }

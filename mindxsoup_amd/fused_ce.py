@@ -9,11 +9,14 @@ them, from the product's exponentials in 16 bits (a piece of the rows at a time)
 backward only multiplies by the gradient that comes from above.  Per-token losses whose table is
 trained are the exception: their gradient needs that factor per row, so the backward runs the
 products anew.
+
+With FEATURES["torch_ops"] (on) the call is the compiled torch.ops.mxs_nf4.head_cross_entropy,
+whose backward runs in C++; FusedHeadCE over ctypes is the other route and gives the same bits.
 """
 
 import torch
 
-from . import _lib, direct
+from . import _lib, direct, ops
 
 REDUCTIONS = ("none", "sum", "mean")
 _DTYPES = {torch.float16: _lib.MXS_DTYPE_F16, torch.bfloat16: _lib.MXS_DTYPE_BF16}
@@ -95,6 +98,25 @@ class FusedHeadCE(torch.autograd.Function):
                 _scaled(dw, grad, ctx.dtypes[1]) if want_dw else None, None, None, None)
 
 
+def _check(hidden, weight, labels):
+    """The operator's own checks, for the other route."""
+    for name, t in (("weight", weight), ("labels", labels)):
+        if t.device != hidden.device:
+            raise ValueError(f"{name} is on {t.device}, hidden on {hidden.device}")
+    if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"hidden [..., D] and weight [V, D], got {tuple(hidden.shape)} and "
+                         f"{tuple(weight.shape)}")
+    if labels.shape != hidden.shape[:-1]:
+        raise ValueError(f"labels {tuple(labels.shape)} for hidden {tuple(hidden.shape)}")
+    if labels.is_floating_point() or labels.is_complex() or labels.dtype == torch.bool:
+        raise ValueError(f"labels must be integers, got {labels.dtype}")
+    if weight.shape[0] == 0 or weight.shape[1] == 0 or weight.shape[1] % 64:
+        raise ValueError(f"the table is [V >= 1, a multiple of 64], got {tuple(weight.shape)}")
+    if hidden.dtype != weight.dtype or hidden.dtype not in _DTYPES:
+        raise ValueError(f"hidden and weight must both be fp16 or both bf16, got {hidden.dtype} "
+                         f"and {weight.dtype}")
+
+
 def head_cross_entropy(hidden, weight, labels, *, ignore_index=-100, reduction="mean"):
     """Cross entropy of the logits hidden @ weight.T against `labels`, as
     torch.nn.functional.cross_entropy gives it on fp32 logits, without holding them.
@@ -112,26 +134,15 @@ def head_cross_entropy(hidden, weight, labels, *, ignore_index=-100, reduction="
     for name, t in (("hidden", hidden), ("weight", weight), ("labels", labels)):
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise ValueError(f"{name} must be a GPU tensor")
-        if t.device != hidden.device:
-            raise ValueError(f"{name} is on {t.device}, hidden on {hidden.device}")
-    if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]:
-        raise ValueError(f"hidden [..., D] and weight [V, D], got {tuple(hidden.shape)} and "
-                         f"{tuple(weight.shape)}")
-    if labels.shape != hidden.shape[:-1]:
-        raise ValueError(f"labels {tuple(labels.shape)} for hidden {tuple(hidden.shape)}")
-    if labels.is_floating_point() or labels.is_complex() or labels.dtype == torch.bool:
-        raise ValueError(f"labels must be integers, got {labels.dtype}")
-    vocab, cols = weight.shape
-    if vocab == 0 or cols == 0 or cols % 64:
-        raise ValueError(f"the table is [V >= 1, a multiple of 64], got {tuple(weight.shape)}")
     if torch.is_autocast_enabled("cuda"):
         kind = torch.get_autocast_dtype("cuda")
         hidden, weight = hidden.to(kind), weight.to(kind)
-    if hidden.dtype != weight.dtype or hidden.dtype not in _DTYPES:
-        raise ValueError(f"hidden and weight must both be fp16 or both bf16, got {hidden.dtype} "
-                         f"and {weight.dtype}")
-    flat = labels.reshape(-1).to(torch.int64).contiguous()
-    loss = direct.run(FusedHeadCE, hidden.reshape(-1, cols), weight, flat, int(ignore_index),
+    if ops.ENABLED:
+        return ops.load().head_cross_entropy(hidden, weight, labels, int(ignore_index),
+                                             REDUCTIONS.index(reduction))
+    _check(hidden, weight, labels)
+    loss = direct.run(FusedHeadCE, hidden.reshape(-1, weight.shape[1]), weight,
+                      labels.reshape(-1).to(torch.int64).contiguous(), int(ignore_index),
                       reduction)
     return loss.view(labels.shape) if reduction == "none" else loss
 

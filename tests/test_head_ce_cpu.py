@@ -46,3 +46,24 @@ def test_c_entries_check_arguments_before_any_launch():
     assert g(None, P, 0, 4, 64, 0, P, None) == -1 and g(P, None, 0, 4, 64, 0, P, None) == -1
     assert g(P, P, 0, 4, 63, 0, P, None) == -4 and g(P, P, 0, 4, 64, 1, P, None) == -2
     assert g(P + 4, P, 0, 4, 64, 0, P, None) == -3 and g(P, P, 0, 0, 64, 0, P, None) == 0
+
+
+def test_meta_shapes_and_gradients():
+    from mindxsoup_amd import ops
+
+    mx = ops.load()
+    h = torch.empty(3, 7, 64, device="meta", dtype=torch.bfloat16, requires_grad=True)
+    w = torch.empty(50, 64, device="meta", dtype=torch.bfloat16, requires_grad=True)
+    y = torch.empty(3, 7, device="meta", dtype=torch.int64)
+    for reduction, shape in ((0, (3, 7)), (1, ()), (2, ())):
+        loss = mx.head_cross_entropy(h, w, y, -100, reduction)
+        assert loss.shape == shape and loss.dtype == torch.float32
+        assert "FusedHeadCE" in loss.grad_fn.name()
+        dh, dw = torch.autograd.grad(loss, (h, w), torch.empty_like(loss))
+        assert dh.shape == h.shape and dw.shape == w.shape
+        assert dh.dtype == dw.dtype == torch.bfloat16
+    with pytest.raises(ValueError, match="multiple of 64"):
+        mx.head_cross_entropy(h[..., :32], w[:, :32], y, -100, 2)
+    with pytest.raises(ValueError, match="GPU"):
+        mx.head_cross_entropy(torch.zeros(2, 64).half(), torch.zeros(5, 64).half(),
+                              torch.zeros(2).long(), -100, 2)

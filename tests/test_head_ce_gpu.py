@@ -307,7 +307,38 @@ def test_autocast(cuda):
     assert da.dtype == db.dtype == torch.float32 and da.any() and db.any()
 
 
-def test_refusals(cuda):
+@pytest.mark.parametrize("trained", [False, True])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_both_routes_give_the_same_bits(cuda, monkeypatch, reduction, trained):
+    """The compiled operator and the Python Function over ctypes."""
+    from mindxsoup_amd import direct, ops
+
+    case = _case(150, 700, 128, F16, ignored=20)
+    assert ops.ENABLED
+    a = _check(*case, reduction=reduction, trained=trained)
+    leaf = case[0].clone().requires_grad_(True)
+    node = fused_ce.head_cross_entropy(leaf, case[1], case[2]).grad_fn
+    assert "FusedHeadCE" in node.name() and type(node).__name__ == "CppFunction"
+    monkeypatch.setattr(ops, "ENABLED", False)
+    for nograd in (False, True):
+        monkeypatch.setattr(direct, "enabled", nograd)
+        b = _check(*case, reduction=reduction, trained=trained)
+        assert torch.equal(a[0], b[0]) and all(map(torch.equal, a[1], b[1]))
+
+
+def test_no_second_derivative(cuda):
+    h, w, y = _case(20, 100, 64, F16)
+    h = h.requires_grad_(True)
+    loss = fused_ce.head_cross_entropy(h, w, y)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(loss, h, create_graph=True)
+
+
+@pytest.mark.parametrize("compiled", [True, False])
+def test_refusals(cuda, monkeypatch, compiled):
+    from mindxsoup_amd import ops
+
+    monkeypatch.setattr(ops, "ENABLED", compiled)
     h, w, y = _case(4, 20, 64, F16)
     run = fused_ce.head_cross_entropy
     for bad in (dict(reduction="max"),):
