@@ -83,6 +83,7 @@ struct CeArgs {
   int mean, per_row;
   // workspace
   int* count;        // rows with a label
+  int* share;        // [2] of dh: shares of the vocabulary, steps of one
   float* gmax;       // largest |row_grad| of them
   int* idx;          // [Tp] their rows in h
   int* lab;          // [Tp] their labels; -1 behind the last, -2 outside the vocabulary
@@ -92,12 +93,15 @@ struct CeArgs {
   float2* stat;      // [blocks][piece rows] power of two and sum of a block of columns
   uint32_t* shift;   // [blocks][piece rows] binades from a block's to its row's power of two
   u32x4* e;          // [Vp / 32][piece rows / 32][2][64] fragments of exponentials, then dz
-  float* part;       // [splits][piece rows][D]
+  float* part;       // [shares][rows in whole tiles of dh][D]
   // the piece
   int row0, rows;    // first gathered row, rows (a multiple of kRowPad)
   int first;         // the call's first piece
-  int stat_cols;     // columns of a block of `stat`
-  int splits, split_steps;
+  int last;          // the call's last piece
+  int stat_cols;     // columns of a block of `stat`; 0: a block is what a wave of a workgroup saw
+  int blocks;        // of `stat`
+  int dh_bm, dh_nx;  // rows of a tile of dh, its column tiles
+  int dh_most, cus;  // workgroups of dh at most; compute units
 };
 
 __device__ __forceinline__ int piece_rows(const CeArgs& a) {
@@ -429,9 +433,10 @@ __device__ __forceinline__ int xcd_place(int b, int n) {
 // ---- logits -----------------------------------------------------------------------------------
 
 // BM rows x kVocabTile columns a tile, WM x (8 / WM) waves.
-template <typename T, int BM, int WM, int NS_, bool KEEP>
+template <typename T, int BM, int WM, int NS_, bool KEEP, bool RANGE>
 struct Logits {
-  static constexpr bool RANGE = BM < 256;
+  // a wave's statistics run on over its workgroup's tiles, where nothing needs them per tile
+  static constexpr bool RUN = RANGE && !KEEP;
   static constexpr int BN = kVocabTile, WN = kWaves / WM, NS = NS_;
   static constexpr int TM = BM / 32 / WM, TN = BN / 32 / WN;
   static constexpr int COLS = 32 * TN;  // columns of a wave: one block of statistics
@@ -449,6 +454,7 @@ struct Logits {
   B cb;
   int wave, lane, mt, wm0, wn0, m_copy;
   int first_col, end;  // of the workgroup's columns, where it has a range of its own
+  float run_top[TM], run_sum[TM];
   bool lean;
 
   __device__ __forceinline__ Logits(const CeArgs& args, const char* lds) : a(args), smem(lds) {
@@ -504,7 +510,7 @@ struct Logits {
   __device__ __forceinline__ void next() const {}
 
   // acc[i][j][r]: row 32 i + lane % 32, column 32 j + 8 (r / 4) + 4 (lane / 32) + r % 4.
-  __device__ __forceinline__ bool done(int q, float16_t (&acc)[TM][TN]) const {
+  __device__ __forceinline__ bool done(int q, float16_t (&acc)[TM][TN]) {
     int v0, m;
     coords(q, v0, m);
     if (v0 >= a.V) return false;
@@ -569,22 +575,48 @@ struct Logits {
         }
       }
       sum += __shfl_xor(sum, 32);
-      if (h == 0) a.stat[(int64_t)(v0 / COLS) * a.rows + row] = make_float2(top, sum);
+      if constexpr (RUN) {
+        const float to = fmaxf(run_top[i], top);
+        run_sum[i] = run_sum[i] * __builtin_amdgcn_exp2f(run_top[i] - to) +
+                     sum * __builtin_amdgcn_exp2f(top - to);
+        run_top[i] = to;
+      } else {
+        if (h == 0) a.stat[(int64_t)(v0 / COLS) * a.rows + row] = make_float2(top, sum);
+      }
     }
     return KEEP;
   }
+  // RUN: the workgroup's waves joined, a block of statistics each
+  __device__ __forceinline__ void finish(char* lds) const {
+    float2* s = reinterpret_cast<float2*>(lds);
+    __syncthreads();  // the stages are done with
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+      if (lane < 32)
+        s[(wave % WN) * BM + wm0 + 32 * i + lane] = make_float2(run_top[i], run_sum[i]);
+    __syncthreads();
+    for (int r = threadIdx.x; r < BM; r += kThreads) {
+      float top = -3e38f, sum = 0.0f;
+      for (int w = 0; w < WN; w++) top = fmaxf(top, s[w * BM + r].x);
+      for (int w = 0; w < WN; w++)
+        sum += s[w * BM + r].y * __builtin_amdgcn_exp2f(s[w * BM + r].x - top);
+      a.stat[(int64_t)blockIdx.x * a.rows + r] = make_float2(top, sum);
+    }
+  }
 };
 
-template <typename T, int BM, int WM, int NS, bool KEEP>
+template <typename T, int BM, int WM, int NS, bool KEEP, bool RANGE>
 __global__ __launch_bounds__(kThreads) void k_ce_logits(CeArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  using P = Logits<T, BM, WM, NS, KEEP>;
+  using P = Logits<T, BM, WM, NS, KEEP, RANGE>;
   P p(a, smem);
   p.mt = (piece_rows(a) + BM - 1) / BM;
   const int g = (int)gridDim.x, wg = p.place(0);
   int tiles = 0;
   p.first_col = 0, p.end = a.V;
-  if constexpr (P::RANGE) {
+  if constexpr (RANGE) {
+#pragma unroll
+    for (int i = 0; i < P::TM; i++) p.run_top[i] = -3e38f, p.run_sum[i] = 0.0f;
     const int blocks = (a.V + P::COLS - 1) / P::COLS, per = (blocks + g - 1) / g * P::COLS;
     p.first_col = wg * per;
     if (p.mt && p.first_col < a.V) {
@@ -596,9 +628,26 @@ __global__ __launch_bounds__(kThreads) void k_ce_logits(CeArgs a) {
     tiles = wg < places ? (places - wg + g - 1) / g : 0;
   }
   if (tiles > 0) stream_tiles<T, P::TM, P::TN>(p, smem, tiles, a.D / kK);
+  if constexpr (P::RUN) p.finish(smem);
 }
 
 // ---- statistics of a row ----------------------------------------------------------------------
+
+// How dh's reduction over the vocabulary is shared out, for the rows that there are: the number of
+// shares that takes the fewest rounds of steps over the compute units, their partial sums' traffic
+// counted in.  (The host knows only how many rows there could be: with a quarter of 1024 rows
+// ignored its shares would leave a quarter of the compute units idle.)
+__device__ __forceinline__ void dh_share(const CeArgs& a, int rows) {
+  const int steps = (a.V + kK - 1) / kK, tiles = (rows + a.dh_bm - 1) / a.dh_bm * a.dh_nx;
+  int best = 0, shares = 1, per = steps;
+  for (int z = 1; z * tiles <= a.dh_most && z <= 64 && (z == 1 || 16 * z <= steps); z++) {
+    const int n = (steps + z - 1) / z;
+    const int cost = (tiles * z + a.cus - 1) / a.cus * (n + 24) + 2 * z;
+    if (z == 1 || cost < best) best = cost, shares = (steps + n - 1) / n, per = n;
+  }
+  a.share[0] = shares;
+  a.share[1] = per;
+}
 
 constexpr int kJoinRows = 8;  // rows of a workgroup, over 128 strips of blocks
 
@@ -612,7 +661,7 @@ __global__ __launch_bounds__(1024) void k_ce_join(CeArgs a) {
   const int n = piece_rows(a), r = threadIdx.x % kJoinRows, strip = threadIdx.x / kJoinRows;
   if ((int)blockIdx.x * kJoinRows >= n) return;
   const int row = (int)blockIdx.x * kJoinRows + r;
-  const int blocks = (a.V + a.stat_cols - 1) / a.stat_cols;
+  const int blocks = a.blocks;
   float top = -3e38f, sum = 0.0f;
   auto join = [&](float t, float s) {
     const float to = fmaxf(top, t);
@@ -632,6 +681,7 @@ __global__ __launch_bounds__(1024) void k_ce_join(CeArgs a) {
   top = -3e38f, sum = 0.0f;
   for (int w = 0; w < 16; w++) join(s_part[w][r].x, s_part[w][r].y);
   if (row >= n) return;
+  if (blockIdx.x == 0 && threadIdx.x == 0 && a.dh) dh_share(a, n);
   if constexpr (SHIFT) {
     constexpr int kBits = sizeof(T) == 2 && Elem<T>::kExpBits > 0 ? 10 : 7;
     constexpr float kMost = kBits == 10 ? 31.0f : 255.0f;
@@ -657,19 +707,23 @@ __global__ __launch_bounds__(1024) void k_ce_join(CeArgs a) {
   if (a.per_row && a.loss) a.loss[a.idx[g]] = st.loss;
 }
 
-__global__ __launch_bounds__(1024) void k_ce_loss(CeArgs a) {
-  __shared__ double s[1024];
-  const int t = threadIdx.x, n = a.count[0];
+// The sum or mean of the losses, in fp64 and a fixed order, by 256 lanes.
+__device__ __forceinline__ void total_loss(const CeArgs& a) {
+  __shared__ double s[4];
+  const int n = a.count[0];
   double x = 0.0;
-  for (int i = t; i < n; i += 1024) x += (double)a.row[i].loss;
-  s[t] = x;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += 256) x += (double)a.row[i].loss;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
   __syncthreads();
-  for (int o = 512; o; o >>= 1) {
-    if (t < o) s[t] += s[t + o];
-    __syncthreads();
-  }
-  if (t == 0) a.loss[0] = (float)(a.mean ? s[0] / (double)n : s[0]);  // 0 / 0 without labels
+  if (threadIdx.x) return;
+  x = s[0] + s[1] + s[2] + s[3];
+  a.loss[0] = (float)(a.mean ? x / (double)n : x);  // 0 / 0 without labels
 }
+
+__global__ __launch_bounds__(256) void k_ce_loss(CeArgs a) { total_loss(a); }
 
 // ---- dz ---------------------------------------------------------------------------------------
 
@@ -740,6 +794,7 @@ struct HiddenGrad {
   B cb;
   const char* ebase;
   int wave, lane, m0, n0, k0, wm0, wn0;
+  int64_t part_row;  // of the share's partial sums: row 0 of the piece
   bool lean;
   int at[TN];
   uint32_t now[TM], then[TM];
@@ -804,7 +859,7 @@ struct HiddenGrad {
     }
   }
   __device__ __forceinline__ bool done(int, float16_t (&acc)[TM][TN]) const {
-    float* out = a.part + (int64_t)(k0 / a.split_steps) * a.rows * a.D;
+    float* out = a.part + part_row * a.D;
 #pragma unroll
     for (int i = 0; i < TM; i++) {
       float* row = out + (int64_t)(m0 + wm0 + 32 * i + (lane & 31)) * a.D;
@@ -826,28 +881,39 @@ struct HiddenGrad {
 // Consecutive places are the column tiles of a row tile, then the row tiles of a share: an XCD's
 // 32 workgroups read few shares' operands (1024 tokens: one share, all of its tiles).
 template <typename T, int BM, int BN, int WM, int NS, bool SHIFT>
-__global__ __launch_bounds__(kThreads) void k_ce_dh(CeArgs a, int nx, int ny) {
+__global__ __launch_bounds__(kThreads) void k_ce_dh(CeArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using P = HiddenGrad<T, BM, BN, WM, NS, SHIFT>;
+  const int ny = (piece_rows(a) + BM - 1) / BM;
+  if (ny == 0) return;
+  const int shares = a.share[0], per = a.share[1], all = shares * ny * a.dh_nx;
+  if ((int)blockIdx.x >= all) return;
   P p(a);
-  const int at = xcd_place((int)blockIdx.x, (int)gridDim.x), x = at % nx, yz = at / nx;
+  const int at = xcd_place((int)blockIdx.x, all), x = at % a.dh_nx, yz = at / a.dh_nx;
   p.m0 = yz % ny * BM;
   p.n0 = x * BN;
-  p.k0 = yz / ny * a.split_steps;
-  const int steps = min((a.V + kK - 1) / kK - p.k0, a.split_steps);
-  if (p.m0 < piece_rows(a)) stream_tiles<T, P::TM, P::TN>(p, smem, 1, steps);
+  p.k0 = yz / ny * per;
+  p.part_row = (int64_t)(yz / ny) * ny * BM;
+  const int steps = min((a.V + kK - 1) / kK - p.k0, per);
+  stream_tiles<T, P::TM, P::TN>(p, smem, 1, steps);
 }
 
 // dh rows = the shares' sum, with the scales, to their places in [T, D].
 template <typename T, bool SHIFT>
 __global__ __launch_bounds__(256) void k_ce_dh_sum(CeArgs a) {
-  const int n = piece_rows(a), row = (int)blockIdx.x;
+  const int n = piece_rows(a), row = (int)blockIdx.x - 1;
+  if (row < 0) {  // one workgroup sums the losses beside the others' work
+    if (blockIdx.y == 0 && a.last && a.loss && !a.per_row) total_loss(a);
+    return;
+  }
   const int d = ((int)blockIdx.y * 256 + (int)threadIdx.x) * 4;
   if (row >= n || d >= a.D) return;
   float4_t x = {0, 0, 0, 0};
   const float* p = a.part + (int64_t)row * a.D + d;
-  for (int z = 0; z < a.splits; z++)
-    x += *reinterpret_cast<const float4_t*>(p + (int64_t)z * a.rows * a.D);
+  const int shares = a.share[0];
+  const int64_t next = (int64_t)(n + a.dh_bm - 1) / a.dh_bm * a.dh_bm * a.D;
+#pragma unroll 4
+  for (int z = 0; z < shares; z++) x += *reinterpret_cast<const float4_t*>(p + z * next);
   const int g = a.row0 + row, i = a.idx[g];
   float f = __builtin_amdgcn_exp2f(-Elem<T>::kGradBits);
   if constexpr (SHIFT) {
@@ -1044,12 +1110,13 @@ static int ce_lds(K fn, int bytes, bool (&set)[16]) {
   return MXS_OK;
 }
 
-// How a call runs: pieces of the rows, tiles and shares.
+// How a call runs: pieces of the rows, tiles.
 struct CePlan {
   int Tp, rows, pieces;   // padded rows, rows of a piece
-  int bm;                 // rows of a logits tile: 256, 128, 64 or 32
+  int bm;                 // rows of a logits tile
   int stat_cols, blocks;
-  int dh_bm, dh_bn, splits, split_steps;
+  int dh_bm, dh_bn;
+  int64_t part_rows;      // of partial sums of dh
   int64_t vp;             // vocabulary in whole tiles
 };
 
@@ -1064,29 +1131,30 @@ static CePlan ce_plan(int T, int V, int D, bool grads, int cus) {
     while (most < p.Tp && most < 8192) most *= 2;  // 8 KB of statistics a row at 128 K columns
   p.pieces = (int)((p.Tp + most - 1) / most);
   p.rows = (int)((p.Tp / kRowPad + p.pieces - 1) / p.pieces) * kRowPad;
-  p.bm = T <= 32 && !grads ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
-  p.stat_cols = p.bm == 256 ? 128 : p.bm == 32 ? 32 : 64;
-  p.blocks = (int)(p.vp / p.stat_cols);
+  // Up to 128 rows one tile holds them; past that tiles of 256, or two of 160 or 192 and three of
+  // 192, where 256 would be a quarter empty (300 rows: 216 us of logits with 256, MEASURED).
+  p.bm = T <= 32 && !grads ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : p.pieces > 1 ? 256
+         : (T > 256 && T <= 320) || (T > 128 && T <= 160) ? 160
+         : (T > 320 && T <= 384) || (T > 512 && T <= 576) || (T > 160 && T <= 192) ? 192 : 256;
+  const bool run = p.bm <= 128 && !grads;
+  p.stat_cols = run ? 0 : p.bm == 256 ? 128 : p.bm == 160 ? 32 : 64;
+  p.blocks = run ? cus : (V + p.stat_cols - 1) / p.stat_cols;
+  // dh: the widest tile whose columns fit, on a part of the compute units' rounds
   p.dh_bm = T <= 64 ? 64 : 256;
-  const int steps = (V + kK - 1) / kK;
-  const int mt = ((p.pieces > 1 ? p.rows : T) + p.dh_bm - 1) / p.dh_bm;
+  const int steps = (V + kK - 1) / kK, rows = p.pieces > 1 ? p.rows : T;
+  const int mt = (rows + p.dh_bm - 1) / p.dh_bm;
   double best = 0;
   for (int bn : {256, 192, 128}) {
     if (bn == 192 && p.dh_bm == 64) continue;  // six column blocks do not share out over the waves
     const int tiles = mt * ((D + bn - 1) / bn);
-    for (int s = 1; s <= 64 && s <= (steps + 15) / 16; s++) {
-      const int per = (steps + s - 1) / s, z = (steps + per - 1) / per;
-      const int rounds = (tiles * z + cus - 1) / cus;
-      // a step's cost by its tile's width, the shares' sums as traffic
+    for (int z = 1; z <= 64 && (z == 1 || (16 * z <= steps && z * tiles <= 2 * cus)); z++) {
+      const int per = (steps + z - 1) / z, rounds = (tiles * z + cus - 1) / cus;
       const double cost = rounds * (per * (0.25 + bn / 256.0) + 24) + 0.5 * z * mt;
-      if (best == 0 || cost < best) {
-        best = cost;
-        p.dh_bn = bn;
-        p.splits = z;
-        p.split_steps = per;
-      }
+      if (best == 0 || cost < best) best = cost, p.dh_bn = bn;
     }
   }
+  const int nx = (D + p.dh_bn - 1) / p.dh_bn;
+  p.part_rows = (int64_t)(mt > 2 * cus / nx ? mt : 2 * cus / nx + 1) * p.dh_bm;
   return p;
 }
 
@@ -1107,23 +1175,24 @@ static CeLayout ce_layout(const CePlan& p, int D, bool grads, bool dh) {
   l.hc = take(2LL * p.Tp * D);
   l.row = take(16LL * p.Tp);
   l.zy = take(4LL * p.Tp);
-  l.stat = take(8LL * p.blocks * p.rows);
-  l.shift = grads ? take(4LL * p.blocks * p.rows) : 0;
+  // (tiles past the vocabulary's last block leave statistics too)
+  const int64_t blocks = p.stat_cols ? p.vp / p.stat_cols : p.blocks;
+  l.stat = take(8LL * blocks * p.rows);
+  l.shift = grads ? take(4LL * blocks * p.rows) : 0;
   l.e = grads ? take(2LL * p.vp * p.rows) : 0;
-  l.part = dh ? take(4LL * p.splits * p.rows * D) : 0;
+  l.part = dh ? take(4LL * p.part_rows * D) : 0;
   l.end = at;
   return l;
 }
 
-template <typename T, int BM, int WM, int NS, bool KEEP>
-static int launch_logits(const CeArgs& a, int cus, hipStream_t stream) {
-  using P = Logits<T, BM, WM, NS, KEEP>;
+template <typename T, int BM, int WM, int NS, bool KEEP, bool RANGE>
+static int launch_logits(const CeArgs& a, hipStream_t stream) {
+  using P = Logits<T, BM, WM, NS, KEEP, RANGE>;
   static bool set[16];
-  auto* fn = &k_ce_logits<T, BM, WM, NS, KEEP>;
+  auto* fn = &k_ce_logits<T, BM, WM, NS, KEEP, RANGE>;
   const int rc = ce_lds(fn, P::LDS, set);
   if (rc != MXS_OK) return rc;
-  const int per_cu = 2 * P::LDS <= 160 * 1024 ? 2 : 1;
-  hipLaunchKernelGGL(fn, dim3(cus * per_cu), dim3(kThreads), P::LDS, stream, a);
+  hipLaunchKernelGGL(fn, dim3(a.cus), dim3(kThreads), P::LDS, stream, a);
   return ce_launched();
 }
 
@@ -1134,10 +1203,7 @@ static int launch_dh(const CeArgs& a, const CePlan& p, hipStream_t stream) {
   auto* fn = &k_ce_dh<T, BM, BN, WM, NS, SHIFT>;
   const int rc = ce_lds(fn, P::LDS, set);
   if (rc != MXS_OK) return rc;
-  const int rows = a.rows < a.T ? a.rows : a.T;
-  const int nx = (a.D + BN - 1) / BN, ny = (rows + BM - 1) / BM;
-  hipLaunchKernelGGL(fn, dim3(nx * ny * p.splits), dim3(kThreads), P::LDS, stream, a, nx,
-                     ny);
+  hipLaunchKernelGGL(fn, dim3(a.dh_most), dim3(kThreads), P::LDS, stream, a);
   return ce_launched();
 }
 
@@ -1159,12 +1225,14 @@ static int launch_dw(const CeArgs& a, int cus, hipStream_t stream) {
   } while (0)
 
 template <typename T, bool KEEP>
-static int logits_of(const CeArgs& a, const CePlan& p, int cus, hipStream_t stream) {
+static int logits_of(const CeArgs& a, const CePlan& p, hipStream_t stream) {
   switch (p.bm) {
-    case 32: return launch_logits<T, 32, 1, 8, KEEP>(a, cus, stream);
-    case 64: return launch_logits<T, 64, 2, 7, KEEP>(a, cus, stream);
-    case 128: return launch_logits<T, 128, 2, 6, KEEP>(a, cus, stream);
-    default: return launch_logits<T, 256, 4, 4, KEEP>(a, cus, stream);
+    case 32: return launch_logits<T, 32, 1, 8, KEEP, true>(a, stream);
+    case 64: return launch_logits<T, 64, 2, 7, KEEP, true>(a, stream);
+    case 128: return launch_logits<T, 128, 2, 6, KEEP, true>(a, stream);
+    case 160: return launch_logits<T, 160, 1, 5, KEEP, false>(a, stream);
+    case 192: return launch_logits<T, 192, 2, 5, KEEP, false>(a, stream);
+    default: return launch_logits<T, 256, 4, 4, KEEP, false>(a, stream);
   }
 }
 
@@ -1195,8 +1263,12 @@ static int run_ce(CeArgs a, const CePlan& p, int cus, hipStream_t stream) {
     a.row0 = i * p.rows;
     a.rows = p.rows < p.Tp - a.row0 ? p.rows : p.Tp - a.row0;
     a.first = i == 0;
-    CE_TRY(grads ? (logits_of<T, true>(a, p, cus, stream))
-                 : (logits_of<T, false>(a, p, cus, stream)));
+    a.last = i + 1 == p.pieces;
+    // tiles that there could be; their shares fill the compute units twice at most
+    const int live = a.T - a.row0 < a.rows ? a.T - a.row0 : a.rows;
+    const int tiles = (live + p.dh_bm - 1) / p.dh_bm * a.dh_nx;
+    a.dh_most = tiles > 2 * cus ? tiles : 2 * cus;
+    CE_TRY(grads ? (logits_of<T, true>(a, p, stream)) : (logits_of<T, false>(a, p, stream)));
     if (shift)
       hipLaunchKernelGGL((k_ce_join<T, true>), dim3(a.rows / kJoinRows), dim3(1024), 0, stream, a);
     else
@@ -1210,7 +1282,7 @@ static int run_ce(CeArgs a, const CePlan& p, int cus, hipStream_t stream) {
     }
     if (a.dh) {
       CE_TRY(shift ? (dh_of<T, true>(a, p, stream)) : (dh_of<T, false>(a, p, stream)));
-      const dim3 grid(a.rows, (a.D / 4 + 255) / 256);
+      const dim3 grid(a.rows + 1, (a.D / 4 + 255) / 256);
       if (shift)
         hipLaunchKernelGGL((k_ce_dh_sum<T, true>), grid, dim3(256), 0, stream, a);
       else
@@ -1218,8 +1290,8 @@ static int run_ce(CeArgs a, const CePlan& p, int cus, hipStream_t stream) {
       CE_TRY(ce_launched());
     }
   }
-  if (a.loss && !a.per_row) {
-    hipLaunchKernelGGL(k_ce_loss, dim3(1), dim3(1024), 0, stream, a);
+  if (a.loss && !a.per_row && !a.dh) {
+    hipLaunchKernelGGL(k_ce_loss, dim3(1), dim3(256), 0, stream, a);
     CE_TRY(ce_launched());
   }
   return MXS_OK;
@@ -1279,8 +1351,9 @@ int mxs_head_ce(const void* h, int64_t ldh, const void* w, int64_t ldw, const in
   a.shift = reinterpret_cast<uint32_t*>(ws + l.shift);
   a.e = reinterpret_cast<u32x4*>(ws + l.e);
   a.part = reinterpret_cast<float*>(ws + l.part);
-  a.stat_cols = p.stat_cols;
-  a.splits = p.splits, a.split_steps = p.split_steps;
+  a.share = reinterpret_cast<int*>(ws + 8);
+  a.stat_cols = p.stat_cols, a.blocks = p.blocks, a.cus = cus;
+  a.dh_bm = p.dh_bm, a.dh_nx = (D + p.dh_bn - 1) / p.dh_bn;
   return dtype == MXS_DTYPE_F16 ? run_ce<_Float16>(a, p, cus, stream)
                                 : run_ce<__bf16>(a, p, cus, stream);
 }

@@ -115,10 +115,12 @@ def _check(h, w, y, reduction="mean", trained=True, scale=3.0, ignore=-100):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("rows", [1, 2, 31, 32, 33, 64, 65, 128, 129, 255, 257, 513])
+@pytest.mark.parametrize("rows", [1, 2, 31, 32, 33, 64, 65, 128, 129, 160, 161, 192, 193, 255,
+                                  257, 320, 321, 384, 385, 513, 576, 577])
 def test_rows(cuda, rows, dtype):
     print(f"case rows={rows} {dtype}", flush=True)
     _check(*_case(rows, 1000, 128, dtype, ignored=rows // 3))
+    _check(*_case(rows, 1000, 128, dtype), trained=False)
 
 
 @pytest.mark.parametrize("trained", [False, True])
