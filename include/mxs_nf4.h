@@ -656,8 +656,17 @@ int mxs_state_values(const void* codes, const float* scale, int64_t n, int is_si
 int64_t mxs_head_ce_workspace_bytes(int T, int V, int D, int want_dh, int want_dw);
 int mxs_head_ce(const void* h, int64_t ldh, const void* w, int64_t ldw, const int64_t* labels,
                 int T, int V, int D, int dtype, int64_t ignore_index, int reduction,
-                const float* row_grad, float* loss, float* dh, float* dw, void* workspace,
-                hipStream_t stream);
+                const float* row_grad, float* loss, float* dh, float* dw, int keep_dz,
+                void* workspace, hipStream_t stream);
+
+/* The table's gradient apart, for calls whose rows are one piece (mxs_head_ce_one_piece: 1 or 0):
+ * mxs_head_ce with keep_dz = 1 (dw NULL) leaves in its workspace what this needs, with the sizes,
+ * dtype, reduction and row_grad of that call and want_dh = whether it had a dh.
+ * dw [V, D] in dtype = that gradient times g[0] (device; NULL: 1), rounded once. */
+int mxs_head_ce_one_piece(int T, int V, int D);
+int mxs_head_ce_table_grad(const void* workspace, int T, int V, int D, int dtype, int reduction,
+                           const float* row_grad, int want_dh, const float* g, void* dw,
+                           hipStream_t stream);
 
 /* out [rows, cols] (fp16 or bf16) = unit (fp32) * g[0], or g[row] with per_row: the gradient that
  * mxs_head_ce left, times the one that came from above.  cols % 8 == 0, 16-byte aligned. */

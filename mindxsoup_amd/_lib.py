@@ -116,7 +116,9 @@ _SIGNATURES = {
                        P, P, P],
     "mxs_state_values": [P, P, I64, I32, P, P],
     "mxs_head_ce_workspace_bytes": [I32, I32, I32, I32, I32],
-    "mxs_head_ce": [P, I64, P, I64, P, I32, I32, I32, I32, I64, I32, P, P, P, P, P, P],
+    "mxs_head_ce": [P, I64, P, I64, P, I32, I32, I32, I32, I64, I32, P, P, P, P, I32, P, P],
+    "mxs_head_ce_one_piece": [I32, I32, I32],
+    "mxs_head_ce_table_grad": [P, I32, I32, I32, I32, I32, P, I32, P, P, P],
     "mxs_head_ce_grad": [P, P, I32, I64, I32, I32, P, P],
 }
 

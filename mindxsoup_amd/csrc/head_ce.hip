@@ -80,6 +80,8 @@ struct CeArgs {
   float* loss;   // [T] or [1]
   float* dh;     // [T, D] or null
   float* dw;     // [V, D] or null
+  void* dw_final;      // [V, D] in the element type, and the factor from above
+  const float* scale;  // (null: 1)
   int mean, per_row;
   // workspace
   int* count;        // rows with a label
@@ -651,8 +653,10 @@ __device__ __forceinline__ void dh_share(const CeArgs& a, int rows) {
 
 constexpr int kJoinRows = 8;  // rows of a workgroup, over 128 strips of blocks
 
-// Joins the blocks' powers of two and sums, all but the label's, and with the label's logit gives
-// the row's loss: log(1 + rest / label), which stays exact for a label that is all but certain.
+// Joins the blocks' powers of two and sums, all but the label's.  With the label's exponential q
+// times smaller than the rest: log-sum-exp = z_y + log(1 + q), and 1 - p_y = q / (1 + q), which the
+// gradient takes, stays exact for a label that is all but certain.  The loss is log-sum-exp rounded
+// to fp32, less z_y: the cross entropy of fp32 logits, with its 2^-24 |z| of rounding.
 // SHIFT: leaves each block's distance to the row's power of two for dh, in both halves of a word
 // and at the place of the exponent in a T.
 template <typename T, bool SHIFT>
@@ -699,7 +703,8 @@ __global__ __launch_bounds__(1024) void k_ce_join(CeArgs a) {
   if (y >= 0 && !(a.zy[g] > 3.4e38f)) {  // (a logit of +inf: NaN, as its exponential is no number)
     const float d = __builtin_fmaf(a.zy[g], kLog2e, -top);  // label's power of two over the rest's
     const float q = sum * __builtin_amdgcn_exp2f(-d);
-    st.loss = d < -60.0f ? kLn2 * (log2f(sum) - d) : log1pf(q);
+    const float more = d < -60.0f ? kLn2 * (log2f(sum) - d) : log1pf(q);
+    st.loss = a.zy[g] < -3.4e38f ? more : (a.zy[g] + more) - a.zy[g];
     st.miss = q > 1e30f ? 1.0f : q / (1.0f + q);
     st.inv = 1.0f / (sum + __builtin_amdgcn_exp2f(d));
   }
@@ -937,27 +942,34 @@ __global__ __launch_bounds__(256) void k_ce_dh_sum(CeArgs a) {
 
 // ---- dW ---------------------------------------------------------------------------------------
 
-// dW [V, D] (+)= dz^T h over the piece's rows: 256 table rows x BN columns a tile.  Both operands
+// dW [V, D] (+)= dz^T h over the piece's rows: 256 table rows x BN columns a tile, in fp32.  FINAL:
+// of a call's only piece, times the factor from above, in T: written once, where the fp32 sums and
+// their rounding would move five times those bytes.  Both operands
 // have the reduction (the rows of h) across their LDS rows: transposing reads.  A block of dz holds
 // 32 rows; in LDS, row t of half b of column block c lies at place t ^ (4 b + 8 (c % 2)), so that
 // the 32 lanes of a read meet all banks.
-template <typename T, int BN, int NS_>
+template <typename T, int BN, int NS_, bool FINAL>
 struct TableGrad {
   static constexpr int BM = 256, WM = 4, WN = 2, NS = NS_, TM = 2, TN = BN / 64;
   using B = ColTile<BN>;
   static constexpr int A_BYTES = BM * kK * 2;
   using A = Share<A_BYTES>;
   static constexpr int STAGE = A_BYTES + B::BYTES, NCP = A::N + B::N;
-  static constexpr int STORES = TM * TN * 4, LDS = NS * STAGE;
+  static constexpr int STORES = TM * TN * (FINAL ? 2 : 4), LDS = NS * STAGE;
   static_assert(A::kEven && B::kEven, "copies per wave");
   static constexpr bool lean = false;
   const CeArgs& a;
   B cb;
   const char* ebase;
   int wave, lane, nt, wm0, wn0;
+  float factor;  // of the sums: kGradBits, row_grad's largest, the mean, FINAL: from above
   int at[TN], eat[2][2];
 
   __device__ __forceinline__ TableGrad(const CeArgs& args) : a(args) {
+    factor = __builtin_amdgcn_exp2f(-Elem<T>::kGradBits);
+    if (a.row_grad) factor *= a.gmax[0];
+    if (a.mean) factor /= (float)max(a.count[0], 1);
+    if (FINAL && a.scale) factor *= a.scale[0];
     wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     lane = threadIdx.x & 63;
     wm0 = wave / WN * 64;
@@ -1012,35 +1024,56 @@ struct TableGrad {
   __device__ __forceinline__ bool done(int q, float16_t (&acc)[TM][TN]) const {
     int v, n;
     coords(q, v, n);
-    float f = __builtin_amdgcn_exp2f(-Elem<T>::kGradBits);
-    if (a.row_grad) f *= a.gmax[0];
-    if (a.mean) f /= (float)max(a.count[0], 1);
 #pragma unroll
     for (int i = 0; i < TM; i++) {
-      const int row = v * BM + wm0 + 32 * i + (lane & 31);
-      if (row >= a.V) continue;
-      float* out = a.dw + (int64_t)row * a.D;
+      const int row = v * BM + wm0 + 32 * i + (lane & 31), h = lane >> 5;
+      const bool out = row >= a.V;
+      const int64_t at = (int64_t)row * a.D;
 #pragma unroll
-      for (int j = 0; j < TN; j++)
+      for (int j = 0; j < TN; j++) {
+        const int d0 = n * BN + wn0 + 32 * j;
+        if constexpr (FINAL) {
+          // the halves of a wave hold columns 8 g .. + 3 and + 4 .. + 7: exchanged, so that a lane
+          // stores eight of them
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-          const int d = n * BN + wn0 + 32 * j + 8 * g + 4 * (lane >> 5);
-          if (d >= a.D) continue;
-          float4_t x;
+          for (int g = 0; g < 4; g += 2) {
+            uint32_t own[2][2];
 #pragma unroll
-          for (int e = 0; e < 4; e++) x[e] = acc[i][j][4 * g + e] * f;
-          if (!a.first) x += *reinterpret_cast<const float4_t*>(out + d);
-          *reinterpret_cast<float4_t*>(out + d) = x;
+            for (int q = 0; q < 2; q++)
+#pragma unroll
+              for (int e = 0; e < 2; e++)
+                own[q][e] = Elem<T>::pack(acc[i][j][4 * (g + q) + 2 * e] * factor,
+                                          acc[i][j][4 * (g + q) + 2 * e + 1] * factor);
+            const uint32_t x = __shfl_xor(h ? own[0][0] : own[1][0], 32);
+            const uint32_t y = __shfl_xor(h ? own[0][1] : own[1][1], 32);
+            const u32x4 w = h ? (u32x4){x, y, own[1][0], own[1][1]}
+                              : (u32x4){own[0][0], own[0][1], x, y};
+            const int d = d0 + 8 * (g + h);
+            if (!out && d < a.D)
+              *reinterpret_cast<u32x4*>(static_cast<T*>(a.dw_final) + at + d) = w;
+          }
+        } else {
+#pragma unroll
+          for (int g = 0; g < 4; g++) {
+            const int d = d0 + 8 * g + 4 * h;
+            if (out || d >= a.D) continue;
+            float4_t x;
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = acc[i][j][4 * g + e] * factor;
+            if (!a.first) x += *reinterpret_cast<const float4_t*>(a.dw + at + d);
+            *reinterpret_cast<float4_t*>(a.dw + at + d) = x;
+          }
         }
+      }
     }
     return (v + 1) * BM <= a.V && (n + 1) * BN <= a.D;  // else some stores fall away
   }
 };
 
-template <typename T, int BN, int NS>
+template <typename T, int BN, int NS, bool FINAL>
 __global__ __launch_bounds__(kThreads) void k_ce_dw(CeArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  using P = TableGrad<T, BN, NS>;
+  using P = TableGrad<T, BN, NS, FINAL>;
   P p(a);
   p.nt = (a.D + BN - 1) / BN;
   const int places = (a.V + P::BM - 1) / P::BM * p.nt, g = (int)gridDim.x;
@@ -1049,7 +1082,7 @@ __global__ __launch_bounds__(kThreads) void k_ce_dw(CeArgs a) {
   if (tiles == 0) return;
   if (steps > 0) {
     stream_tiles<T, P::TM, P::TN>(p, smem, tiles, steps);
-  } else if (a.first) {  // no row has a label
+  } else if (FINAL || a.first) {  // no row has a label
     float16_t acc[P::TM][P::TN] = {};
     for (int q = 0; q < tiles; q++) p.done(q, acc);
   }
@@ -1132,7 +1165,7 @@ static CePlan ce_plan(int T, int V, int D, bool grads, int cus) {
   p.pieces = (int)((p.Tp + most - 1) / most);
   p.rows = (int)((p.Tp / kRowPad + p.pieces - 1) / p.pieces) * kRowPad;
   // Up to 128 rows one tile holds them; past that tiles of 256, or two of 160 or 192 and three of
-  // 192, where 256 would be a quarter empty (300 rows: 216 us of logits with 256, MEASURED).
+  // 192, where 256 would be a quarter empty (301 rows, a call: 202 us; with tiles of 256 230).
   p.bm = T <= 32 && !grads ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : p.pieces > 1 ? 256
          : (T > 256 && T <= 320) || (T > 128 && T <= 160) ? 160
          : (T > 320 && T <= 384) || (T > 512 && T <= 576) || (T > 160 && T <= 192) ? 192 : 256;
@@ -1207,14 +1240,15 @@ static int launch_dh(const CeArgs& a, const CePlan& p, hipStream_t stream) {
   return ce_launched();
 }
 
-template <typename T, int BN, int NS>
-static int launch_dw(const CeArgs& a, int cus, hipStream_t stream) {
-  using P = TableGrad<T, BN, NS>;
+template <typename T, bool FINAL>
+static int launch_dw(const CeArgs& a, hipStream_t stream) {
+  constexpr int BN = 256, NS = 4;
+  using P = TableGrad<T, BN, NS, FINAL>;
   static bool set[16];
-  auto* fn = &k_ce_dw<T, BN, NS>;
+  auto* fn = &k_ce_dw<T, BN, NS, FINAL>;
   const int rc = ce_lds(fn, P::LDS, set);
   if (rc != MXS_OK) return rc;
-  hipLaunchKernelGGL(fn, dim3(cus), dim3(kThreads), P::LDS, stream, a);
+  hipLaunchKernelGGL(fn, dim3(a.cus), dim3(kThreads), P::LDS, stream, a);
   return ce_launched();
 }
 
@@ -1249,16 +1283,17 @@ static int dh_of(const CeArgs& a, const CePlan& p, hipStream_t stream) {
 }
 
 template <typename T>
-static int run_ce(CeArgs a, const CePlan& p, int cus, hipStream_t stream) {
-  const bool grads = a.dh || a.dw;
+static int run_ce(CeArgs a, const CePlan& p, bool keep_dz, hipStream_t stream) {
+  const bool want_dz = a.dw || keep_dz, grads = a.dh || want_dz;
+  const int cus = a.cus;
   const int vec = (uintptr_t)a.h % 16 == 0 && a.ldh % 8 == 0;
   hipLaunchKernelGGL(k_ce_rows, dim3(p.Tp / kGather), dim3(256), 0, stream, a, vec);
   CE_TRY(ce_launched());
-  if (a.dw && a.row_grad) {
+  if (want_dz && a.row_grad) {
     hipLaunchKernelGGL(k_ce_gmax, dim3(1), dim3(1024), 0, stream, a);
     CE_TRY(ce_launched());
   }
-  const bool shift = a.dh && !a.dw;
+  const bool shift = a.dh && !want_dz;
   for (int i = 0; i < p.pieces; i++) {
     a.row0 = i * p.rows;
     a.rows = p.rows < p.Tp - a.row0 ? p.rows : p.Tp - a.row0;
@@ -1274,11 +1309,11 @@ static int run_ce(CeArgs a, const CePlan& p, int cus, hipStream_t stream) {
     else
       hipLaunchKernelGGL((k_ce_join<T, false>), dim3(a.rows / kJoinRows), dim3(1024), 0, stream, a);
     CE_TRY(ce_launched());
-    if (a.dw) {
+    if (want_dz) {
       const int tbs = a.rows / 32, ys = 4096 / tbs + 1;
       hipLaunchKernelGGL(k_ce_dz<T>, dim3(tbs, ys), dim3(256), 0, stream, a);
       CE_TRY(ce_launched());
-      CE_TRY((launch_dw<T, 256, 4>(a, cus, stream)));
+      if (a.dw) CE_TRY((launch_dw<T, false>(a, stream)));
     }
     if (a.dh) {
       CE_TRY(shift ? (dh_of<T, true>(a, p, stream)) : (dh_of<T, false>(a, p, stream)));
@@ -1315,33 +1350,17 @@ int64_t mxs_head_ce_workspace_bytes(int T, int V, int D, int want_dh, int want_d
   return ce_layout(ce_plan(T > 0 ? T : 1, V, D, grads, ce_cus()), D, grads, want_dh != 0).end;
 }
 
-int mxs_head_ce(const void* h, int64_t ldh, const void* w, int64_t ldw, const int64_t* labels,
-                int T, int V, int D, int dtype, int64_t ignore_index, int reduction,
-                const float* row_grad, float* loss, float* dh, float* dw, void* workspace,
-                hipStream_t stream) {
+int mxs_head_ce_one_piece(int T, int V, int D) {
   const int rc = ce_sizes(T, V, D);
   if (rc != MXS_OK) return rc;
-  if (dtype != MXS_DTYPE_F16 && dtype != MXS_DTYPE_BF16) return MXS_ERR_DTYPE;
-  if (!w || !workspace || (T && (!h || !labels || (!loss && !dh && !dw))))
-    return MXS_ERR_ARG;
-  if (reduction < 0 || reduction > 2 || ldh < D || ldw < D) return MXS_ERR_ARG;
-  if (T && dw && reduction == 0 && !row_grad) return MXS_ERR_ARG;
-  if ((uintptr_t)w % 16 || ldw % 8 || (uintptr_t)workspace % 256) return MXS_ERR_ALIGN;
-  if ((uintptr_t)dh % 16 || (uintptr_t)dw % 16) return MXS_ERR_ALIGN;
-  // offsets within a tile are 32 bits
-  if (ldw > (1 << 22) || ldh > ((int64_t)1 << 40)) return MXS_ERR_SIZE;
-  const int cus = ce_cus();
-  const bool grads = dh || dw;
-  const CePlan p = ce_plan(T > 0 ? T : 1, V, D, grads, cus);
-  const CeLayout l = ce_layout(p, D, grads, dh != nullptr);
-  char* ws = static_cast<char*>(workspace);
-  CeArgs a = {};
-  a.h = h, a.ldh = ldh, a.w = w, a.ldw = ldw, a.labels = labels, a.ignore = ignore_index;
-  a.T = T, a.V = V, a.D = D, a.row_grad = row_grad, a.loss = loss, a.dh = dh, a.dw = dw;
-  a.per_row = reduction == 0;
-  a.mean = reduction == 2;
+  return ce_plan(T > 0 ? T : 1, V, D, true, ce_cus()).pieces == 1;
+}
+
+// The workspace's places.
+static void ce_places(CeArgs& a, const CePlan& p, const CeLayout& l, char* ws, int cus) {
   a.count = reinterpret_cast<int*>(ws);
   a.gmax = reinterpret_cast<float*>(ws + 4);
+  a.share = reinterpret_cast<int*>(ws + 8);
   a.idx = reinterpret_cast<int*>(ws + l.idx);
   a.lab = reinterpret_cast<int*>(ws + l.lab);
   a.hc = ws + l.hc;
@@ -1351,11 +1370,59 @@ int mxs_head_ce(const void* h, int64_t ldh, const void* w, int64_t ldw, const in
   a.shift = reinterpret_cast<uint32_t*>(ws + l.shift);
   a.e = reinterpret_cast<u32x4*>(ws + l.e);
   a.part = reinterpret_cast<float*>(ws + l.part);
-  a.share = reinterpret_cast<int*>(ws + 8);
   a.stat_cols = p.stat_cols, a.blocks = p.blocks, a.cus = cus;
-  a.dh_bm = p.dh_bm, a.dh_nx = (D + p.dh_bn - 1) / p.dh_bn;
-  return dtype == MXS_DTYPE_F16 ? run_ce<_Float16>(a, p, cus, stream)
-                                : run_ce<__bf16>(a, p, cus, stream);
+  a.dh_bm = p.dh_bm, a.dh_nx = (a.D + p.dh_bn - 1) / p.dh_bn;
+}
+
+int mxs_head_ce(const void* h, int64_t ldh, const void* w, int64_t ldw, const int64_t* labels,
+                int T, int V, int D, int dtype, int64_t ignore_index, int reduction,
+                const float* row_grad, float* loss, float* dh, float* dw, int keep_dz,
+                void* workspace, hipStream_t stream) {
+  const int rc = ce_sizes(T, V, D);
+  if (rc != MXS_OK) return rc;
+  if (dtype != MXS_DTYPE_F16 && dtype != MXS_DTYPE_BF16) return MXS_ERR_DTYPE;
+  if (!w || !workspace || (T && (!h || !labels || (!loss && !dh && !dw && !keep_dz))))
+    return MXS_ERR_ARG;
+  if (reduction < 0 || reduction > 2 || ldh < D || ldw < D) return MXS_ERR_ARG;
+  if (T && (dw || keep_dz) && reduction == 0 && !row_grad) return MXS_ERR_ARG;
+  if (dw && keep_dz) return MXS_ERR_ARG;
+  if ((uintptr_t)w % 16 || ldw % 8 || (uintptr_t)workspace % 256) return MXS_ERR_ALIGN;
+  if ((uintptr_t)dh % 16 || (uintptr_t)dw % 16) return MXS_ERR_ALIGN;
+  // offsets within a tile are 32 bits
+  if (ldw > (1 << 22) || ldh > ((int64_t)1 << 40)) return MXS_ERR_SIZE;
+  const int cus = ce_cus();
+  const bool grads = dh || dw || keep_dz;
+  const CePlan p = ce_plan(T > 0 ? T : 1, V, D, grads, cus);
+  if (keep_dz && p.pieces > 1) return MXS_ERR_SIZE;
+  const CeLayout l = ce_layout(p, D, grads, dh != nullptr);
+  CeArgs a = {};
+  a.h = h, a.ldh = ldh, a.w = w, a.ldw = ldw, a.labels = labels, a.ignore = ignore_index;
+  a.T = T, a.V = V, a.D = D, a.row_grad = row_grad, a.loss = loss, a.dh = dh, a.dw = dw;
+  a.per_row = reduction == 0;
+  a.mean = reduction == 2;
+  ce_places(a, p, l, static_cast<char*>(workspace), cus);
+  return dtype == MXS_DTYPE_F16 ? run_ce<_Float16>(a, p, keep_dz != 0, stream)
+                                : run_ce<__bf16>(a, p, keep_dz != 0, stream);
+}
+
+int mxs_head_ce_table_grad(const void* workspace, int T, int V, int D, int dtype, int reduction,
+                           const float* row_grad, int want_dh, const float* g, void* dw,
+                           hipStream_t stream) {
+  const int rc = ce_sizes(T, V, D);
+  if (rc != MXS_OK) return rc;
+  if (dtype != MXS_DTYPE_F16 && dtype != MXS_DTYPE_BF16) return MXS_ERR_DTYPE;
+  if (!workspace || !dw || reduction < 0 || reduction > 2) return MXS_ERR_ARG;
+  if ((uintptr_t)dw % 16 || (uintptr_t)workspace % 256) return MXS_ERR_ALIGN;
+  const int cus = ce_cus();
+  const CePlan p = ce_plan(T > 0 ? T : 1, V, D, true, cus);
+  if (p.pieces > 1) return MXS_ERR_SIZE;
+  CeArgs a = {};
+  a.T = T, a.V = V, a.D = D, a.row_grad = row_grad, a.mean = reduction == 2;
+  ce_places(a, p, ce_layout(p, D, true, want_dh != 0),
+            static_cast<char*>(const_cast<void*>(workspace)), cus);
+  a.rows = p.rows, a.first = 1, a.scale = g, a.dw_final = dw;
+  return dtype == MXS_DTYPE_F16 ? launch_dw<_Float16, true>(a, stream)
+                                : launch_dw<__bf16, true>(a, stream);
 }
 
 int mxs_head_ce_grad(const float* unit, const float* g, int per_row, int64_t rows, int cols,

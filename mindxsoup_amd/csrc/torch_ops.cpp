@@ -18,7 +18,7 @@
 //   lora_bwd_group    lora_bwd for them, small launches shared
 //   mlp_fwd, mlp_bwd  the SwiGLU MLP block of three such projections (solution/mlp.py:33-44)
 //   grad_norm, adamw_step, state_values  the end of a training step over lists of tensors
-//   head_ce, head_ce_grad  the head's cross entropy and its gradients (solution/fused_ce.py:95-148)
+//   head_ce, head_ce_grad, head_ce_table_grad  the head's cross entropy and its gradients (solution/fused_ce.py:95-148)
 // Autograd ops (one node per call; backward in C++), named as the package's Python Functions
 // they stand for (a node's name() says which ran):
 //   linear         NF4LinearFunction
@@ -1767,7 +1767,10 @@ HeadCe head_ce_meta(const Tensor& h, const Tensor& w, const Tensor& labels, int6
   Tensor loss, dh, dw;
   if (want_loss) loss = reduction == 0 ? at::empty({h.size(0)}, f32) : at::empty({}, f32);
   if (want_dh) dh = at::empty(h.sizes(), f32);
-  if (want_dw) dw = at::empty(w.sizes(), f32);
+  const int T = as_int(h.size(0), "T"), D = as_int(h.size(1), "D"), V = as_int(w.size(0), "V");
+  if (want_dw && mxs_head_ce_one_piece(T, V, D) == 1)  // the workspace
+    dw = at::empty({mxs_head_ce_workspace_bytes(T, V, D, want_dh, 1)}, f32.dtype(at::kByte));
+  else if (want_dw) dw = at::empty(w.sizes(), f32);
   return {loss, dh, dw};
 }
 
@@ -1786,14 +1789,19 @@ HeadCe head_ce_cuda(const Tensor& h, const Tensor& w, const Tensor& labels, int6
   }
   const Tensor y = labels.to(at::kLong).contiguous();
   const Tensor g = row_grad.has_value() && row_grad->defined() ? row_grad->contiguous() : Tensor();
-  const int64_t bytes = mxs_head_ce_workspace_bytes(T, V, D, want_dh, want_dw);
-  TORCH_CHECK(bytes >= 0, "hidden ", h.sizes(), " and weight ", w.sizes(), ": ",
-              why(static_cast<int>(bytes)));
-  Tensor ws = at::empty({bytes}, h.options().dtype(at::kByte));
+  const bool keep = want_dw && std::get<2>(out).scalar_type() == at::kByte;
+  Tensor ws = std::get<2>(out);
+  if (!keep) {
+    const int64_t bytes = mxs_head_ce_workspace_bytes(T, V, D, want_dh, want_dw);
+    TORCH_CHECK(bytes >= 0, "hidden ", h.sizes(), " and weight ", w.sizes(), ": ",
+                why(static_cast<int>(bytes)));
+    ws = at::empty({bytes}, h.options().dtype(at::kByte));
+  }
   ok(mxs_head_ce(hr.data_ptr(), ldh, wr.data_ptr(), ldw, y.data_ptr<int64_t>(), T, V, D,
                  float_dtype(h, "hidden"), ignore_index, static_cast<int>(reduction),
                  ptr<float>(g), ptr<float>(std::get<0>(out)), ptr<float>(std::get<1>(out)),
-                 ptr<float>(std::get<2>(out)), ws.data_ptr(), stream_of(h)),
+                 keep ? nullptr : ptr<float>(std::get<2>(out)), keep, ws.data_ptr(),
+                 stream_of(h)),
      "mxs_head_ce");
   return out;
 }
@@ -1818,6 +1826,50 @@ Tensor head_ce_grad_cuda(const Tensor& unit, const Tensor& g, at::ScalarType dty
   return out;
 }
 
+const float* row_values(const OptTensor& t, int64_t rows, const at::Device& dev) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->numel() == rows &&
+                  t->device() == dev,
+              "row_grad must be fp32 [", rows, "], got ", t->sizes());
+  return t->data_ptr<float>();
+}
+
+// The table's gradient in `dtype` from head_ce's: fp32 [V, D], or the workspace of a call whose
+// rows are one piece; times g.
+Tensor head_ce_table_grad_meta(const Tensor& dw, int64_t T, int64_t V, int64_t D,
+                               at::ScalarType dtype, int64_t, const OptTensor&, bool,
+                               const OptTensor& g) {
+  if (g.has_value() && g->defined())
+    TORCH_CHECK(g->scalar_type() == at::kFloat && g->numel() == 1 && g->device() == dw.device(),
+                "g must be one fp32 value, got ", g->sizes());
+  TORCH_CHECK(T >= 0 && V > 0 && D > 0, "sizes ", T, ", ", V, ", ", D);
+  return at::empty({V, D}, dw.options().dtype(dtype));
+}
+
+Tensor head_ce_table_grad_cuda(const Tensor& dw, int64_t T, int64_t V, int64_t D,
+                               at::ScalarType dtype, int64_t reduction, const OptTensor& row_grad,
+                               bool want_dh, const OptTensor& g) {
+  const at::OptionalDeviceGuard guard(dw.device());
+  if (dw.scalar_type() != at::kByte) {
+    TORCH_CHECK(dw.sizes() == at::IntArrayRef({V, D}), "dw must be [", V, ", ", D, "]");
+    return g.has_value() && g->defined() ? head_ce_grad_cuda(dw, *g, dtype) : dw.to(dtype);
+  }
+  Tensor out = head_ce_table_grad_meta(dw, T, V, D, dtype, reduction, row_grad, want_dh, g);
+  const int t = as_int(T, "T"), v = as_int(V, "V"), d = as_int(D, "D");
+  TORCH_CHECK(dw.is_contiguous() &&
+                  dw.numel() == mxs_head_ce_workspace_bytes(t, v, d, want_dh, 1),
+              "dw is no workspace of these sizes");
+  ok(mxs_head_ce_table_grad(dw.data_ptr(), t, v, d, float_dtype(out, "the gradient"),
+                            static_cast<int>(reduction),
+                            row_values(row_grad, T, dw.device()),
+                            want_dh, scalar_ptr(g, dw.device(), "g"), out.data_ptr(),
+                            stream_of(dw)),
+     "mxs_head_ce_table_grad");
+  return out;
+}
+
+using HeadCeTableSig = Tensor(const Tensor&, int64_t, int64_t, int64_t, at::ScalarType, int64_t,
+                              const OptTensor&, bool, const OptTensor&);
 using HeadCeSig = HeadCe(const Tensor&, const Tensor&, const Tensor&, int64_t, int64_t,
                          const OptTensor&, bool, bool, bool);
 
@@ -1840,6 +1892,8 @@ struct FusedHeadCE : public torch::autograd::Function<FusedHeadCE> {
     ctx->saved_data["reduction"] = reduction;
     ctx->saved_data["shape"] = hidden.sizes().vec();
     ctx->saved_data["dtype"] = hidden.scalar_type();
+    ctx->saved_data["table"] = weight.sizes().vec();
+    ctx->saved_data["want_dh"] = want_dh;
     if (again) ctx->save_for_backward({hidden, weight, labels});
     else ctx->save_for_backward({dh, dw});
     return reduction == 0 ? loss.view(labels.sizes()) : loss;
@@ -1849,6 +1903,7 @@ struct FusedHeadCE : public torch::autograd::Function<FusedHeadCE> {
     static auto run = op<HeadCeSig>("mxs_nf4::head_ce");
     static auto scale =
         op<Tensor(const Tensor&, const Tensor&, at::ScalarType)>("mxs_nf4::head_ce_grad");
+    static auto table = op<HeadCeTableSig>("mxs_nf4::head_ce_table_grad");
     TORCH_CHECK(!at::GradMode::is_enabled(), "head_cross_entropy has no second derivative");
     const auto saved = ctx->get_saved_variables();
     const bool wh = ctx->needs_input_grad(0), ww = ctx->needs_input_grad(1);
@@ -1857,17 +1912,24 @@ struct FusedHeadCE : public torch::autograd::Function<FusedHeadCE> {
     at::AutoDispatchBelowADInplaceOrView below;
     Tensor g = grads[0].to(at::kFloat), dh, dw;
     if (reduction == 0) g = g.reshape({-1}).contiguous();
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    const auto size = ctx->saved_data["table"].toIntVector();
+    int64_t rows = 1;
+    for (size_t i = 0; i + 1 < shape.size(); i++) rows *= shape[i];
     if (ctx->saved_data["again"].toBool()) {
       std::tie(std::ignore, dh, dw) =
           run.call(rows2d(saved[0]), saved[1], saved[2].reshape({-1}),
                    ctx->saved_data["ignore"].toInt(), reduction, g, false, wh, ww);
       if (dh.defined()) dh = dh.to(dtype);
-      if (dw.defined()) dw = dw.to(dtype);
+      if (ww)
+        dw = table.call(dw, rows, size[0], size[1], dtype, reduction, g, wh, std::nullopt);
     } else {
       if (wh) dh = scale.call(saved[0], g, dtype);
-      if (ww) dw = scale.call(saved[1], g, dtype);
+      if (ww)
+        dw = table.call(saved[1], rows, size[0], size[1], dtype, reduction, std::nullopt,
+                        ctx->saved_data["want_dh"].toBool(), g);
     }
-    if (dh.defined()) dh = dh.view(ctx->saved_data["shape"].toIntVector());
+    if (dh.defined()) dh = dh.view(shape);
     return {dh, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
@@ -1957,6 +2019,8 @@ TORCH_LIBRARY(mxs_nf4, m) {
         "Tensor? row_grad, bool want_loss, bool want_dh, bool want_dw) "
         "-> (Tensor, Tensor, Tensor)");
   m.def("head_ce_grad(Tensor unit, Tensor g, ScalarType dtype) -> Tensor");
+  m.def("head_ce_table_grad(Tensor dw, int T, int V, int D, ScalarType dtype, int reduction, "
+        "Tensor? row_grad, bool want_dh, Tensor? g) -> Tensor");
   m.def("head_cross_entropy(Tensor hidden, Tensor weight, Tensor labels, int ignore_index, "
         "int reduction) -> Tensor");
 }
@@ -1976,6 +2040,7 @@ TORCH_LIBRARY_IMPL(mxs_nf4, CUDA, m) {
   m.impl("state_values", &state_values_cuda);
   m.impl("head_ce", &head_ce_cuda);
   m.impl("head_ce_grad", &head_ce_grad_cuda);
+  m.impl("head_ce_table_grad", &head_ce_table_grad_cuda);
 }
 
 TORCH_LIBRARY_IMPL(mxs_nf4, Meta, m) {
@@ -1993,6 +2058,7 @@ TORCH_LIBRARY_IMPL(mxs_nf4, Meta, m) {
   m.impl("state_values", &state_values_meta);
   m.impl("head_ce", &head_ce_meta);
   m.impl("head_ce_grad", &head_ce_grad_meta);
+  m.impl("head_ce_table_grad", &head_ce_table_grad_meta);
 }
 
 // The autograd ops: the same node with or without grad mode (without it, or with no input

@@ -5,10 +5,12 @@ works through it in chunks).
     loss = fused_ce.head_cross_entropy(hidden, lm_head.weight, labels)
 
 The losses take one product with the table; where gradients are wanted the forward also computes
-them, from the product's exponentials in 16 bits (a piece of the rows at a time), and the
-backward only multiplies by the gradient that comes from above.  Per-token losses whose table is
-trained are the exception: their gradient needs that factor per row, so the backward runs the
-products anew.
+that of the hidden states, from the product's exponentials in 16 bits (a piece of the rows at a
+time), and the backward multiplies it by the gradient that comes from above.  A trained table's
+gradient is the backward's own product where the rows are one piece, over dz kept from the forward
+(16 bits, 1 GiB at most); of several pieces it is summed in fp32 beside them.  Per-token losses
+whose table is trained need the factor from above per row, so their backward runs all products
+anew.
 
 With FEATURES["torch_ops"] (on) the call is the compiled torch.ops.mxs_nf4.head_cross_entropy,
 whose backward runs in C++; FusedHeadCE over ctypes is the other route and gives the same bits.
@@ -33,7 +35,8 @@ def _rows(t, cols):
 
 
 def _run(h, w, labels, ignore_index, reduction, row_grad, want_loss, want_dh, want_dw):
-    """One call of mxs_head_ce: (loss, dh, dw), None where not wanted."""
+    """One call of mxs_head_ce: (loss, dh, dw), None where not wanted.  dw: fp32 [V, D], or, of one
+    piece's rows, the workspace that _table_grad makes it from."""
     rows, cols = h.shape
     vocab, dev = w.shape[0], h.device
     f32 = dict(dtype=torch.float32, device=dev)
@@ -42,18 +45,34 @@ def _run(h, w, labels, ignore_index, reduction, row_grad, want_loss, want_dh, wa
         w, ldw = _rows(w, cols)
         if ldw % 8 or w.data_ptr() % 16:
             w, ldw = w.clone(memory_format=torch.contiguous_format), cols
+        L = _lib.lib()
+        keep = bool(want_dw) and L.mxs_head_ce_one_piece(rows, vocab, cols) == 1
         loss = torch.empty(rows if reduction == "none" else (), **f32) if want_loss else None
         dh = torch.empty(rows, cols, **f32) if want_dh else None
-        dw = torch.empty(vocab, cols, **f32) if want_dw else None
-        n = _lib.lib().mxs_head_ce_workspace_bytes(rows, vocab, cols, want_dh, want_dw)
+        dw = torch.empty(vocab, cols, **f32) if want_dw and not keep else None
+        n = L.mxs_head_ce_workspace_bytes(rows, vocab, cols, want_dh, want_dw)
         if n < 0:
             _lib.check(n, "mxs_head_ce_workspace_bytes")
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
         _lib.call("mxs_head_ce", _lib.ptr(h), ldh, _lib.ptr(w), ldw, _lib.ptr(labels), rows,
                   vocab, cols, _DTYPES[h.dtype], ignore_index, REDUCTIONS.index(reduction),
-                  _lib.ptr(row_grad), _lib.ptr(loss), _lib.ptr(dh), _lib.ptr(dw), _lib.ptr(ws),
-                  _lib.stream_of(dev))
-    return loss, dh, dw
+                  _lib.ptr(row_grad), _lib.ptr(loss), _lib.ptr(dh), _lib.ptr(dw), int(keep),
+                  _lib.ptr(ws), _lib.stream_of(dev))
+    return loss, dh, ws if keep else dw
+
+
+def _table_grad(dw, h, w_shape, reduction, row_grad, want_dh, g):
+    """The table's gradient in h's dtype from what _run left for it, times g (one value or None)."""
+    if dw.dtype != torch.uint8:
+        return dw.to(h.dtype) if g is None else _scaled(dw, g, h.dtype)
+    out = torch.empty(w_shape, dtype=h.dtype, device=dw.device)
+    if g is not None:
+        g = g.to(torch.float32).contiguous()
+    with torch.cuda.device(dw.device):
+        _lib.call("mxs_head_ce_table_grad", _lib.ptr(dw), h.shape[0], w_shape[0], w_shape[1],
+                  _DTYPES[h.dtype], REDUCTIONS.index(reduction), _lib.ptr(row_grad),
+                  int(want_dh), _lib.ptr(g), _lib.ptr(out), _lib.stream_of(dw.device))
+    return out
 
 
 def _scaled(unit, g, dtype):
@@ -76,26 +95,30 @@ class FusedHeadCE(torch.autograd.Function):
         again = want_dw and reduction == "none"
         loss, dh, dw = _run(hidden, weight, labels, ignore_index, reduction, None, True,
                             want_dh and not again, want_dw and not again)
-        ctx.again, ctx.args = again, (ignore_index, reduction)
-        ctx.dtypes = hidden.dtype, weight.dtype
+        ctx.again, ctx.args, ctx.w_shape = again, (ignore_index, reduction), weight.shape
+        ctx.want_dh = want_dh
         if again:
             ctx.save_for_backward(hidden, weight, labels)
         else:
-            ctx.save_for_backward(dh, dw)
+            ctx.save_for_backward(hidden.new_empty(hidden.shape[0], 0), dh, dw)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         want_dh, want_dw = ctx.needs_input_grad[:2]
+        reduction = ctx.args[1]
         if ctx.again:
-            grad = grad.to(torch.float32).contiguous()
+            hidden, grad = ctx.saved_tensors[0], grad.to(torch.float32).contiguous()
             _, dh, dw = _run(*ctx.saved_tensors, *ctx.args, grad, False, want_dh, want_dw)
-            return (dh.to(ctx.dtypes[0]) if want_dh else None,
-                    dw.to(ctx.dtypes[1]) if want_dw else None, None, None, None)
-        dh, dw = ctx.saved_tensors
-        return (_scaled(dh, grad, ctx.dtypes[0]) if want_dh else None,
-                _scaled(dw, grad, ctx.dtypes[1]) if want_dw else None, None, None, None)
+            dh = dh.to(hidden.dtype) if want_dh else None
+            if want_dw:
+                dw = _table_grad(dw, hidden, ctx.w_shape, reduction, grad, want_dh, None)
+            return dh, dw, None, None, None
+        hidden, dh, dw = ctx.saved_tensors  # hidden: its type and rows
+        return (_scaled(dh, grad, hidden.dtype) if want_dh else None,
+                _table_grad(dw, hidden, ctx.w_shape, reduction, None, ctx.want_dh, grad)
+                if want_dw else None, None, None, None)
 
 
 def _check(hidden, weight, labels):

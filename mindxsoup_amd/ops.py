@@ -22,7 +22,7 @@ PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmxs_nf4_torc
 OPS = ("dequant", "linear_fwd", "linear_bwd_dx", "lora_fwd", "lora_bwd", "lora_fwd_group",
        "lora_bwd_group", "linear", "lora_linear", "lora_siblings", "mlp_fwd", "mlp_bwd",
        "grad_norm", "adamw_step", "state_values", "head_ce", "head_ce_grad",
-       "head_cross_entropy")
+       "head_ce_table_grad", "head_cross_entropy")
 
 # set by apply() from FEATURES["torch_ops"]; False: the Python Functions.  Off when MXS_NF4_LIB
 # names another build of the C-ABI library: this library links the package's own copy by file

@@ -31,8 +31,9 @@ def test_c_entries_check_arguments_before_any_launch():
     P = 0x10000
 
     def run(h=P, ldh=64, w=P, ldw=64, y=P, T=4, V=10, D=64, dt=0, red=2, rg=None, loss=P, dh=P,
-            dw=P, ws=P):
-        return L.mxs_head_ce(h, ldh, w, ldw, y, T, V, D, dt, -100, red, rg, loss, dh, dw, ws, None)
+            dw=P, keep=0, ws=P):
+        return L.mxs_head_ce(h, ldh, w, ldw, y, T, V, D, dt, -100, red, rg, loss, dh, dw, keep, ws,
+                             None)
 
     assert run(h=None) == -1 and run(w=None) == -1 and run(y=None) == -1 and run(ws=None) == -1
     assert run(loss=None, dh=None, dw=None) == -1 and run(red=3) == -1 and run(T=-1) == -1
@@ -42,6 +43,16 @@ def test_c_entries_check_arguments_before_any_launch():
     assert run(dt=1) == -2 and run(dt=7) == -2
     assert run(ldw=68) == -3 and run(w=P + 2) == -3 and run(dh=P + 4) == -3
     assert run(ws=P + 16) == -3 and run(dw=P + 8) == -3
+    assert run(keep=1) == -1 and run(dw=None, keep=1, red=0) == -1
+    assert run(dw=None, keep=1, T=4096, V=1 << 20) == -4  # several pieces
+    assert L.mxs_head_ce_one_piece(2048, 151936, 1536) == 1
+    assert L.mxs_head_ce_one_piece(2049, 151936, 1536) == 0
+    t = L.mxs_head_ce_table_grad
+    assert t(None, 4, 10, 64, 0, 2, None, 1, P, P, None) == -1
+    assert t(P, 4, 10, 64, 0, 2, None, 1, P, None, None) == -1
+    assert t(P, 4, 10, 64, 1, 2, None, 1, P, P, None) == -2
+    assert t(P, 4, 10, 64, 0, 2, None, 1, P, P + 8, None) == -3
+    assert t(P, 4096, 1 << 20, 64, 0, 2, None, 1, P, P, None) == -4
     g = L.mxs_head_ce_grad
     assert g(None, P, 0, 4, 64, 0, P, None) == -1 and g(P, None, 0, 4, 64, 0, P, None) == -1
     assert g(P, P, 0, 4, 63, 0, P, None) == -4 and g(P, P, 0, 4, 64, 1, P, None) == -2

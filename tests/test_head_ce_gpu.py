@@ -328,6 +328,34 @@ def test_both_routes_give_the_same_bits(cuda, monkeypatch, reduction, trained):
         assert torch.equal(a[0], b[0]) and all(map(torch.equal, a[1], b[1]))
 
 
+@pytest.mark.parametrize("compiled", [True, False])
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("vocab", [700, 151936])  # at 2100 rows: one piece, two pieces
+def test_one_of_two_gradients(cuda, monkeypatch, reduction, vocab, compiled):
+    """Of a trained table either gradient alone is what it is beside the other, whether the other
+    input needs none or is only not asked for: the same bits, but for the hidden states' alone
+    under per-row losses, which then takes the route of a frozen table."""
+    from mindxsoup_amd import ops
+
+    monkeypatch.setattr(ops, "ENABLED", compiled)
+    h, w, y = _case(2100, vocab, 64, BF16, ignored=50)
+    g = torch.ones((), device="cuda") if reduction == "mean" else torch.rand(2100, device="cuda")
+
+    def grads(a, b, leaves):
+        loss = fused_ce.head_cross_entropy(a, b, y, reduction=reduction)
+        return torch.autograd.grad(loss, leaves, g, retain_graph=True)
+
+    hh, ww = h.requires_grad_(True), w.requires_grad_(True)
+    dh, dw = grads(hh, ww, (hh, ww))
+    assert torch.equal(grads(hh, ww, (ww,))[0], dw)
+    alone = grads(hh, ww, (hh,))[0]
+    if reduction == "mean":
+        assert torch.equal(alone, dh)
+    else:
+        _within(alone, _exact(hh.detach(), ww.detach(), y, reduction, g)[1], "dh alone")
+    assert torch.equal(grads(hh.detach(), ww, (ww,))[0], dw)
+
+
 def test_no_second_derivative(cuda):
     h, w, y = _case(20, 100, 64, F16)
     h = h.requires_grad_(True)
