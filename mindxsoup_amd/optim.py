@@ -190,6 +190,13 @@ class AdamW(torch.optim.Optimizer):
                        max_norm=self.max_grad_norm, grad_scale=grad_scale, found_inf=found_inf)
         return loss
 
+    def __setstate__(self, state):
+        """Groups of another AdamW's checkpoint get this one's own settings."""
+        super().__setstate__(state)
+        for group in self.param_groups:
+            group.setdefault("state_bits", 32)
+            group.setdefault("min_8bit_size", 4096)
+
     def load_state_dict(self, state_dict):
         """As Optimizer's, but states keep their own types (Optimizer would give them the
         parameter's), and parameters with the same step count share one step tensor again."""
@@ -209,7 +216,8 @@ class AdamW(torch.optim.Optimizer):
                     self.state[p][name] = steps[kind]
                 elif isinstance(value, torch.Tensor):
                     if not name.endswith("_scale"):  # laid out like the parameter
-                        own = torch.empty_like(p, dtype=value.dtype,
+                        dtype = torch.uint8 if value.dtype == torch.uint8 else torch.float32
+                        own = torch.empty_like(p, dtype=dtype,
                                                memory_format=torch.preserve_format)
                         own.copy_(value)
                     else:

@@ -356,6 +356,37 @@ def test_one_of_two_gradients(cuda, monkeypatch, reduction, vocab, compiled):
     assert torch.equal(grads(hh.detach(), ww, (ww,))[0], dw)
 
 
+def test_inference_and_no_grad(cuda):
+    h, w, y = _case(300, 700, 128, F16, ignored=20)
+    want = fused_ce.head_cross_entropy(h, w, y, reduction="none")
+    w.requires_grad_(True)
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            got = fused_ce.head_cross_entropy(h, w, y, reduction="none")
+        assert torch.equal(got, want) and not got.requires_grad
+
+
+def test_more_rows_than_a_grid_side_and_than_a_piece(cuda):
+    """70001 rows of a small vocabulary, in pieces of the row limit; against the losses and gradients
+    of the same rows in two calls, which are independent of one another row by row."""
+    h, w, y = _case(70001, 300, 64, F16, ignored=1000)
+    g = torch.rand(70001, device="cuda")
+
+    def run(a, b, f):
+        a = a.detach().requires_grad_(True)
+        loss = fused_ce.head_cross_entropy(a, w, b, reduction="none")
+        return loss.detach(), torch.autograd.grad(loss, a, f)[0]
+
+    loss, dh = run(h, y, g)
+    for part in (slice(0, 40000), slice(40000, 70001)):
+        l, d = run(h[part], y[part], g[part])
+        assert torch.equal(l, loss[part])
+        # the same dz; the shares of the vocabulary may differ with the rows, and with them the
+        # order of fp32 sums, of at most 300 terms, before the one rounding to fp16
+        off = (d.float() - dh[part].float()).abs()
+        assert bool((off <= 2.0 ** -10 * d.float().abs() + 300 * U * 8 + 2.0 ** -24).all())
+
+
 def test_no_second_derivative(cuda):
     h, w, y = _case(20, 100, 64, F16)
     h = h.requires_grad_(True)

@@ -469,3 +469,81 @@ def test_grad_scaler_hands_over_scale_and_overflow(cuda):
     scaler.update()
     assert torch.equal(p, before) and scaler.get_scale() == 128.0
     assert float(a.state[p]["step"]) == 1.0
+
+
+def test_checkpoint_of_torchs_adamw(cuda):
+    """States of torch's optimizer, in the parameters' type and with a step count each, carry on."""
+    torch.manual_seed(2)
+    a = torch.nn.Parameter(torch.randn(500, device=cuda).bfloat16())
+    theirs = torch.optim.AdamW([a], lr=1e-2)
+    for t in range(2):
+        a.grad = _randn(500, 1.0, t, torch.bfloat16)
+        theirs.step()
+    b, c = (torch.nn.Parameter(a.detach().clone()) for _ in range(2))
+    mine = optim.AdamW([b], lr=1e-2)
+    mine.load_state_dict(copy.deepcopy(theirs.state_dict()))
+    st = theirs.state[a]
+    assert mine.state[b]["exp_avg"].dtype == torch.float32
+    assert torch.equal(mine.state[b]["exp_avg"], st["exp_avg"].float())
+    assert float(mine.state[b]["step"]) == 2.0
+    want = _exact(b.detach(), _randn(500, 1.0, 9, torch.bfloat16), st["exp_avg"], st["exp_avg_sq"],
+                  3, 1e-2, (0.9, 0.999), 1e-8, 1e-2)
+    b.grad = _randn(500, 1.0, 9, torch.bfloat16)
+    mine.step()
+    assert ((b.double() - want[0]).abs() <= want[3] + 2.0 ** -8 * want[0].abs()).all()
+
+
+def test_scaled_gradients_are_clipped_by_their_true_norm(cuda):
+    """GradScaler's factor with max_grad_norm: as the unscaled gradients clipped; the scale is a
+    power of two, so the two differ only where fp32 rounds the coefficient's products."""
+    x = _randn(3000, 1.0, 4)
+    ps = [torch.nn.Parameter(torch.ones(3000, device=cuda)) for _ in range(2)]
+    a, b = (optim.AdamW([p], lr=0.1, eps=1e-3, max_grad_norm=0.5) for p in ps)
+    scaler = torch.amp.GradScaler("cuda", init_scale=1024.0)
+    scaler.scale((ps[0] * x).sum()).backward()
+    scaler.step(a)
+    ps[1].grad = x.clone()
+    b.step()
+    assert torch.equal(a.grad_norm, b.grad_norm)
+    assert (ps[0] - ps[1]).abs().max().item() <= 8 * U
+
+
+def test_more_than_2_to_the_31_values(cuda):
+    """One tensor of 2^31 + 300 values: past 32 bits of offsets and into a second table entry."""
+    n = (1 << 31) + 300
+    g = torch.zeros(n, device=cuda, dtype=torch.bfloat16)
+    at = [0, 5, (1 << 31) - 1, 1 << 31, n - 1]
+    for k, i in enumerate(at):
+        g[i] = 2.0 ** k
+    want = sum(4.0 ** k for k in range(5)) ** 0.5
+    assert abs(optim.grad_norm([g]).item() - want) <= 2 * U * want
+    p = torch.ones(n, device=cuda, dtype=torch.bfloat16)
+    m, v, sm, sv = optim.zero_state8(p)
+    optim.adamw_step([p], [g], [m], [v], torch.zeros((), device=cuda), lr=0.5, eps=1e-6,
+                     betas=(0.9, 0.99), weight_decay=0.0, scales=([sm], [sv]))
+    # a first step moves a parameter by lr wherever there is a gradient: 1 -> 0.5
+    assert torch.equal(p[at].float().cpu(), torch.full((5,), 0.5))
+    p[at] = 1.0
+    assert bool((p == 1.0).all())
+    tail = optim.state_values(m[-300:].clone(), sm[-2:], True)
+    full = optim.state_values(m, sm, True)
+    assert torch.equal(full[-300:], tail) and full[n - 1] == sm[-1] and sm[-1] > 1.0
+
+
+def test_norm_and_step_of_two_calls_at_once(cuda):
+    """Calls on two streams keep their workspaces apart."""
+    cases = [_case(torch.float32, [70000, 11]) for _ in range(2)]
+    want = copy.deepcopy(cases)
+    for p, g, m, v in want:
+        optim.adamw_step(p, g, m, v, torch.zeros((), device=cuda), norm=optim.grad_norm(g),
+                         max_norm=0.1, **ARGS)
+    steps = [torch.zeros((), device=cuda) for _ in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for s, (p, g, m, v), step in zip(streams, cases, steps):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            optim.adamw_step(p, g, m, v, step, norm=optim.grad_norm(g), max_norm=0.1, **ARGS)
+    torch.cuda.synchronize()
+    for a, b in zip(cases, want):
+        for x, y in zip(a, b):
+            assert all(map(torch.equal, x, y))
