@@ -11,21 +11,43 @@
 
 namespace {
 
-std::vector<at::Tensor> list(PyObject* obj, const char* name) {
-  TORCH_CHECK_TYPE(PyList_Check(obj), name, " must be a list of tensors");
-  const Py_ssize_t n = PyList_GET_SIZE(obj);
-  std::vector<at::Tensor> out;
-  out.reserve(n);
-  for (Py_ssize_t i = 0; i < n; i++) {
-    PyObject* x = PyList_GET_ITEM(obj, i);
-    TORCH_CHECK_TYPE(THPVariable_Check(x), name, "[", i, "] must be a tensor, got ",
-                     Py_TYPE(x)->tp_name);
-    const at::Tensor& t = THPVariable_Unpack(x);
-    TORCH_CHECK_VALUE(t.is_cuda(), name, "[", i, "] must be a GPU tensor, found ", t.device());
-    out.push_back(t);
+// The tensors of a Python list, borrowed: the list keeps them alive for the call, so their
+// reference counts stay as they are (two atomic operations a tensor saved).
+class List {
+ public:
+  List(PyObject* obj, const char* name) {
+    TORCH_CHECK_TYPE(PyList_Check(obj), name, " must be a list of tensors");
+    const Py_ssize_t n = PyList_GET_SIZE(obj);
+    tensors_.reserve(n);
+    for (Py_ssize_t i = 0; i < n; i++) {
+      PyObject* x = PyList_GET_ITEM(obj, i);
+      bool good = THPVariable_Check(x);
+      if (good) {
+        const at::Tensor& t = THPVariable_Unpack(x);
+        good = t.is_cuda();
+        if (good) tensors_.push_back(c10::MaybeOwnedTraits<at::Tensor>::createBorrow(t));
+      }
+      if (!good) {
+        release();
+        TORCH_CHECK_TYPE(THPVariable_Check(x), name, "[", i, "] must be a tensor, got ",
+                         Py_TYPE(x)->tp_name);
+        TORCH_CHECK_VALUE(false, name, "[", i, "] must be a GPU tensor, found ",
+                          THPVariable_Unpack(x).device());
+      }
+    }
   }
-  return out;
-}
+  ~List() { release(); }
+  List(const List&) = delete;
+  List& operator=(const List&) = delete;
+  operator at::TensorList() const { return tensors_; }
+
+ private:
+  void release() {
+    for (at::Tensor& t : tensors_) c10::MaybeOwnedTraits<at::Tensor>::destroyBorrow(t);
+    tensors_.clear();
+  }
+  std::vector<at::Tensor> tensors_;
+};
 
 std::optional<at::Tensor> maybe(PyObject* obj, const char* name) {
   if (obj == Py_None) return std::nullopt;
@@ -37,7 +59,8 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
   PyObject *grads, *scale;
   if (!PyArg_ParseTuple(args, "OO", &grads, &scale)) return nullptr;
-  return THPVariable_Wrap(mxs_lists::grad_norm(list(grads, "grads"), maybe(scale, "grad_scale")));
+  const List g(grads, "grads");
+  return THPVariable_Wrap(mxs_lists::grad_norm(g, maybe(scale, "grad_scale")));
   END_HANDLE_TH_ERRORS
 }
 
@@ -54,9 +77,10 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
   o.norm = maybe(norm, "norm");
   o.grad_scale = maybe(scale, "grad_scale");
   o.found_inf = maybe(found, "found_inf");
-  mxs_lists::adamw_step(list(p, "params"), list(g, "grads"), list(m, "exp_avgs"),
-                        list(v, "exp_avg_sqs"), list(ms, "exp_avg_scales"),
-                        list(vs, "exp_avg_sq_scales"), THPVariable_Unpack(step), o);
+  const List params(p, "params"), grads(g, "grads"), avgs(m, "exp_avgs"),
+      avg_sqs(v, "exp_avg_sqs"), scales(ms, "exp_avg_scales"), sq_scales(vs, "exp_avg_sq_scales");
+  mxs_lists::adamw_step(params, grads, avgs, avg_sqs, scales, sq_scales, THPVariable_Unpack(step),
+                        o);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }

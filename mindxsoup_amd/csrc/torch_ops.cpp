@@ -1957,12 +1957,14 @@ Tensor head_cross_entropy_plain(const Tensor& hidden, const Tensor& weight, cons
 namespace mxs_lists {
 
 Tensor grad_norm(TensorList grads, const OptTensor& grad_scale) {
+  at::AutoDispatchBelowADInplaceOrView below;  // nothing here is recorded
   return grad_norm_cuda(grads, grad_scale);
 }
 
 void adamw_step(TensorList params, TensorList grads, TensorList avgs, TensorList avg_sqs,
                 TensorList avg_scales, TensorList avg_sq_scales, const Tensor& step,
                 const StepOptions& o) {
+  at::AutoDispatchBelowADInplaceOrView below;
   adamw_step_cuda(params, grads, avgs, avg_sqs, avg_scales, avg_sq_scales, step, o.lr, o.lr_dev,
                   o.beta1, o.beta2, o.eps, o.weight_decay, o.norm, o.max_norm, o.grad_scale,
                   o.found_inf);

@@ -28,19 +28,21 @@ def _on_gpu(tensors, name):
             raise ValueError(f"{name} takes GPU tensors")
 
 
-@torch.no_grad()
+def _list(tensors):
+    return tensors if type(tensors) is list else list(tensors)
+
+
 def grad_norm(grads, grad_scale=None):
     """The 2-norm over all values of the tensors `grads` (fp32, fp16 or bf16, mixed or not), an
     fp32 scalar tensor on their device; divided by `grad_scale` (one fp32 value on the device,
     the loss scale the gradients still carry) where that is given.  Squares and sums are fp64, in
     a fixed order."""
-    grads = list(grads)
+    grads = _list(grads)
     if not grads:
         raise ValueError("grad_norm takes at least one gradient")
     return ops.lists().grad_norm(grads, grad_scale)
 
 
-@torch.no_grad()
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.999), eps=1e-8,
                weight_decay=0.01, scales=None, norm=None, max_norm=None, grad_scale=None,
                found_inf=None):
@@ -60,8 +62,6 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
     norm: `grad_norm` of the (unscaled) gradients; max_norm: the clipping bound, needed with it.
     lr: a number, or one fp32 value on the device.  grad_scale, found_inf: as GradScaler hands
     them to a fused optimizer; found_inf != 0 leaves parameters, states and step as they were."""
-    params, grads = list(params), list(grads)
-    exp_avgs, exp_avg_sqs = list(exp_avgs), list(exp_avg_sqs)
     _on_gpu([step], "adamw_step")
     if (norm is None) != (max_norm is None):
         raise ValueError("norm and max_norm are given together or not at all")
@@ -71,8 +71,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
     if not eps >= 0.0 or not weight_decay >= 0.0 or (max_norm is not None and not max_norm > 0.0):
         raise ValueError(f"eps {eps}, weight_decay {weight_decay}, max_norm {max_norm}")
     lr_dev = lr if isinstance(lr, torch.Tensor) else None
-    ms, vs = ([], []) if scales is None else map(list, scales)
-    ops.lists().adamw_step(params, grads, exp_avgs, exp_avg_sqs, ms, vs, step,
+    ms, vs = ([], []) if scales is None else map(_list, scales)
+    ops.lists().adamw_step(_list(params), _list(grads), _list(exp_avgs), _list(exp_avg_sqs), ms,
+                           vs, step,
                            0.0 if lr_dev is not None else float(lr), lr_dev, float(b1),
                            float(b2), float(eps), float(weight_decay), norm,
                            1.0 if max_norm is None else float(max_norm), grad_scale, found_inf)
