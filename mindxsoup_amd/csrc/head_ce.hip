@@ -22,7 +22,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kK = 32;             // reduction step: two MFMAs of 16
-constexpr int kWaves = 8;
+constexpr int kWaves = 8;          // of a workgroup, but for narrow tiles of the logits
 constexpr int kThreads = 64 * kWaves;
 constexpr int kRowPad = 256;       // gathered rows are padded with zeros to a multiple of this
 constexpr int kVocabTile = 256;    // vocabulary columns of a logits tile
@@ -227,24 +227,24 @@ __device__ __forceinline__ u32x2 read_tr(const char* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)p));
 }
 
-// Copies of one operand's stage: pieces of 1 KB, piece wave + 8 i copy i of a wave.  Where they do
-// not share out evenly, the waves behind the last piece have one copy less.
-template <int BYTES>
+// Copies of one operand's stage by W waves: pieces of 1 KB, piece wave + W i copy i of a wave.
+// Where they do not share out evenly, the waves behind the last piece have one copy less.
+template <int BYTES, int W = kWaves>
 struct Share {
-  static constexpr int PIECES = BYTES / 1024, N = (PIECES + kWaves - 1) / kWaves;
-  static constexpr bool kEven = PIECES % kWaves == 0;
+  static constexpr int PIECES = BYTES / 1024, N = (PIECES + W - 1) / W;
+  static constexpr bool kEven = PIECES % W == 0;
   __device__ __forceinline__ static bool mine(int i, int wave) {
-    return kEven || i + 1 < N || wave + kWaves * i < PIECES;
+    return kEven || i + 1 < N || wave + W * i < PIECES;
   }
 };
 
 // An operand [ROWS][kK] whose reduction index is contiguous.  64-byte LDS rows of four 16-byte
 // segments, segment s of row r at s ^ (r / 4 % 4): 16 rows of a fragment read then fall on all
 // banks.  A fragment: row lane % 32, reduction indexes 8 (lane / 32) .. + 7 of its 16.
-template <int ROWS>
-struct RowTile : Share<ROWS * kK * 2> {
+template <int ROWS, int W = kWaves>
+struct RowTile : Share<ROWS * kK * 2, W> {
   static constexpr int BYTES = ROWS * kK * 2;
-  using Share<BYTES>::N;
+  using Share<BYTES, W>::N;
   uint32_t off[N];
   const char* base;
 
@@ -253,14 +253,14 @@ struct RowTile : Share<ROWS * kK * 2> {
                                        int lane) {
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      const int row = (wave + kWaves * i) * 16 + (lane >> 2);
+      const int row = (wave + W * i) * 16 + (lane >> 2);
       const int seg = (lane & 3) ^ ((row >> 2) & 3);
       off[i] = ((uint32_t)min(row, last - row0) * (uint32_t)ld + seg * 8) * 2;
     }
     base = static_cast<const char*>(src) + (int64_t)row0 * ld * 2;
   }
   __device__ __forceinline__ void copy(uint32_t lds, int k, int i, int wave) const {
-    copy1k(lds + (wave + kWaves * i) * 1024, base + (int64_t)k * (kK * 2), off[i]);
+    copy1k(lds + (wave + W * i) * 1024, base + (int64_t)k * (kK * 2), off[i]);
   }
   __device__ __forceinline__ static u32x4 read(const char* s, int row0, int kk, int lane) {
     const int row = row0 + (lane & 31);
@@ -332,9 +332,10 @@ struct ColTile : Share<COLS * kK * 2> {
 //   load(s), next()       what fix needs of the step in the stage at s: read, then taken over
 //   done(q, acc)          tile q's sums; acc[i][j] = first_j x second_i; whether this wave issued
 //                         P::STORES stores or more
-// P::NS stages of one 32-deep step each, so that P::NS - 1 steps' copies are under way: with two
-// stages of 64 the copies had less than a step to land, and a step of dh at 256 x 192 took 1.6 us
-// instead of the 0.64 of its products.  A step's second half is multiplied behind the barrier that
+// P::NS stages of one 32-deep step each, so that P::NS - 1 steps' copies are under way.  Large
+// products, which the card's power bounds (1.6 of 2.4 GHz), take the same time with two stages of
+// 64; few rows, which wait for their copies, and stores that drain beside later steps want the
+// many stages.  A step's second half is multiplied behind the barrier that
 // ends it, over the next step's first reads; the stage that this barrier frees takes the copies
 // of the step after P::NS, over that half and the next step's first one.
 // Waits count what was issued after the copies they wait for (vmcnt retires in order): the copies
@@ -434,16 +435,16 @@ __device__ __forceinline__ int xcd_place(int b, int n) {
 
 // ---- logits -----------------------------------------------------------------------------------
 
-// BM rows x kVocabTile columns a tile, WM x (8 / WM) waves.
-template <typename T, int BM, int WM, int NS_, bool KEEP, bool RANGE>
+// BM rows x BN columns a tile, WM x (W / WM) waves.
+template <typename T, int BM, int BN_, int W, int WM, int NS_, bool KEEP, bool RANGE>
 struct Logits {
   // a wave's statistics run on over its workgroup's tiles, where nothing needs them per tile
   static constexpr bool RUN = RANGE && !KEEP;
-  static constexpr int BN = kVocabTile, WN = kWaves / WM, NS = NS_;
+  static constexpr int BN = BN_, WN = W / WM, NS = NS_;
   static constexpr int TM = BM / 32 / WM, TN = BN / 32 / WN;
   static constexpr int COLS = 32 * TN;  // columns of a wave: one block of statistics
-  using A = RowTile<BM>;
-  using B = RowTile<BN>;
+  using A = RowTile<BM, W>;
+  using B = RowTile<BN, W>;
   static constexpr int STAGE = A::BYTES + B::BYTES, NCP = A::N + B::N;
   // Labels of a tile's rows, copied with its first step: a load in the epilogue would wait for
   // every copy before it.  With two steps a tile at least the copies are (NS + 1) / 2 tiles ahead.
@@ -597,7 +598,7 @@ struct Logits {
       if (lane < 32)
         s[(wave % WN) * BM + wm0 + 32 * i + lane] = make_float2(run_top[i], run_sum[i]);
     __syncthreads();
-    for (int r = threadIdx.x; r < BM; r += kThreads) {
+    for (int r = threadIdx.x; r < BM; r += 64 * W) {
       float top = -3e38f, sum = 0.0f;
       for (int w = 0; w < WN; w++) top = fmaxf(top, s[w * BM + r].x);
       for (int w = 0; w < WN; w++)
@@ -607,10 +608,10 @@ struct Logits {
   }
 };
 
-template <typename T, int BM, int WM, int NS, bool KEEP, bool RANGE>
-__global__ __launch_bounds__(kThreads) void k_ce_logits(CeArgs a) {
+template <typename T, int BM, int BN, int W, int WM, int NS, bool KEEP, bool RANGE>
+__global__ __launch_bounds__(64 * W) void k_ce_logits(CeArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  using P = Logits<T, BM, WM, NS, KEEP, RANGE>;
+  using P = Logits<T, BM, BN, W, WM, NS, KEEP, RANGE>;
   P p(a, smem);
   p.mt = (piece_rows(a) + BM - 1) / BM;
   const int g = (int)gridDim.x, wg = p.place(0);
@@ -1147,6 +1148,7 @@ static int ce_lds(K fn, int bytes, bool (&set)[16]) {
 struct CePlan {
   int Tp, rows, pieces;   // padded rows, rows of a piece
   int bm;                 // rows of a logits tile
+  bool narrow;            // of 64 columns instead of 256
   int stat_cols, blocks;
   int dh_bm, dh_bn;
   int64_t part_rows;      // of partial sums of dh
@@ -1169,10 +1171,17 @@ static CePlan ce_plan(int T, int V, int D, bool grads, int cus) {
   p.bm = T <= 32 && !grads ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : p.pieces > 1 ? 256
          : (T > 256 && T <= 320) || (T > 128 && T <= 160) ? 160
          : (T > 320 && T <= 384) || (T > 512 && T <= 576) || (T > 160 && T <= 192) ? 192 : 256;
+  // A small table gives a workgroup 64 columns or fewer.  Tiles that wide take a quarter of the LDS
+  // a stage, and with more stages under way a step waits less for its operands.  Losses alone, a
+  // call, with tiles of 256 columns and with these: 1 row, 5359 columns of 1536: 23.9, 20.6 us;
+  // 11 rows, 5359 of 3264: 39.6, 32.7; 128 rows, 16384 of 4096: 77.0, 48.2.
+  p.narrow = T <= 128 && V <= 64 * cus;
+  if (p.narrow && p.bm == 32) p.bm = 64;
   const bool run = p.bm <= 128 && !grads;
-  p.stat_cols = run ? 0 : p.bm == 256 ? 128 : p.bm == 160 ? 32 : 64;
+  p.stat_cols = run ? 0 : p.bm == 256 ? 128 : p.bm == 160 || p.narrow ? 32 : 64;
   p.blocks = run ? cus : (V + p.stat_cols - 1) / p.stat_cols;
-  // dh: the widest tile whose columns fit, on a part of the compute units' rounds
+  // dh: the tile whose rounds over the compute units take least, each step's fixed part and the
+  // shares' partial sums counted in
   p.dh_bm = T <= 64 ? 64 : 256;
   const int steps = (V + kK - 1) / kK, rows = p.pieces > 1 ? p.rows : T;
   const int mt = (rows + p.dh_bm - 1) / p.dh_bm;
@@ -1218,14 +1227,14 @@ static CeLayout ce_layout(const CePlan& p, int D, bool grads, bool dh) {
   return l;
 }
 
-template <typename T, int BM, int WM, int NS, bool KEEP, bool RANGE>
+template <typename T, int BM, int BN, int W, int WM, int NS, bool KEEP, bool RANGE>
 static int launch_logits(const CeArgs& a, hipStream_t stream) {
-  using P = Logits<T, BM, WM, NS, KEEP, RANGE>;
+  using P = Logits<T, BM, BN, W, WM, NS, KEEP, RANGE>;
   static bool set[16];
-  auto* fn = &k_ce_logits<T, BM, WM, NS, KEEP, RANGE>;
+  auto* fn = &k_ce_logits<T, BM, BN, W, WM, NS, KEEP, RANGE>;
   const int rc = ce_lds(fn, P::LDS, set);
   if (rc != MXS_OK) return rc;
-  hipLaunchKernelGGL(fn, dim3(a.cus), dim3(kThreads), P::LDS, stream, a);
+  hipLaunchKernelGGL(fn, dim3(a.cus), dim3(64 * W), P::LDS, stream, a);
   return ce_launched();
 }
 
@@ -1260,13 +1269,16 @@ static int launch_dw(const CeArgs& a, hipStream_t stream) {
 
 template <typename T, bool KEEP>
 static int logits_of(const CeArgs& a, const CePlan& p, hipStream_t stream) {
+  if (p.narrow)
+    return p.bm == 64 ? launch_logits<T, 64, 64, 4, 2, 12, KEEP, true>(a, stream)
+                      : launch_logits<T, 128, 64, 8, 4, 10, KEEP, true>(a, stream);
   switch (p.bm) {
-    case 32: return launch_logits<T, 32, 1, 8, KEEP, true>(a, stream);
-    case 64: return launch_logits<T, 64, 2, 7, KEEP, true>(a, stream);
-    case 128: return launch_logits<T, 128, 2, 6, KEEP, true>(a, stream);
-    case 160: return launch_logits<T, 160, 1, 5, KEEP, false>(a, stream);
-    case 192: return launch_logits<T, 192, 2, 5, KEEP, false>(a, stream);
-    default: return launch_logits<T, 256, 4, 4, KEEP, false>(a, stream);
+    case 32: return launch_logits<T, 32, 256, 8, 1, 8, KEEP, true>(a, stream);
+    case 64: return launch_logits<T, 64, 256, 8, 2, 7, KEEP, true>(a, stream);
+    case 128: return launch_logits<T, 128, 256, 8, 2, 6, KEEP, true>(a, stream);
+    case 160: return launch_logits<T, 160, 256, 8, 1, 5, KEEP, false>(a, stream);
+    case 192: return launch_logits<T, 192, 256, 8, 2, 5, KEEP, false>(a, stream);
+    default: return launch_logits<T, 256, 256, 8, 4, 4, KEEP, false>(a, stream);
   }
 }
 

@@ -131,6 +131,15 @@ def test_vocabularies(cuda, vocab, trained):
     _check(*_case(300, vocab, 192, BF16), trained=trained)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [1, 33, 64, 65, 128])
+@pytest.mark.parametrize("vocab", [5023, 16384, 16385, 70001])
+def test_few_rows_of_tables(cuda, vocab, rows, dtype):
+    """Tables of 64 columns a compute unit and fewer, and larger ones: each has tiles of its own."""
+    print(f"case vocab={vocab} rows={rows} {dtype}", flush=True)
+    _check(*_case(rows, vocab, 192, dtype, ignored=rows // 3), trained=False)
+
+
 @pytest.mark.parametrize("cols", [64, 128, 192, 256, 320, 448, 1536, 4096])
 def test_widths(cuda, cols):
     print(f"case cols={cols}", flush=True)
