@@ -11,6 +11,21 @@
 
 namespace {
 
+// What the dispatcher would have resolved before a kernel: subclasses that handle operators
+// themselves (sharded and fake tensors), negated views, zeros without memory.  Their memory is not
+// their values, and there is no dispatcher here to see to it.
+bool plain(const at::Tensor& t) {
+  constexpr c10::DispatchKeySet odd({c10::DispatchKey::Python, c10::DispatchKey::Negative,
+                                     c10::DispatchKey::ZeroTensor,
+                                     c10::DispatchKey::Functionalize});
+  return !t.key_set().has_any(odd);
+}
+
+void check_plain(const at::Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(plain(t), name, " must be a tensor that holds its values itself, got one with ",
+                    t.key_set());
+}
+
 // The tensors of a Python list, borrowed: the list keeps them alive for the call, so their
 // reference counts stay as they are (two atomic operations a tensor saved).
 class List {
@@ -24,15 +39,16 @@ class List {
       bool good = THPVariable_Check(x);
       if (good) {
         const at::Tensor& t = THPVariable_Unpack(x);
-        good = t.is_cuda();
+        good = t.is_cuda() && plain(t);
         if (good) tensors_.push_back(c10::MaybeOwnedTraits<at::Tensor>::createBorrow(t));
       }
       if (!good) {
         release();
         TORCH_CHECK_TYPE(THPVariable_Check(x), name, "[", i, "] must be a tensor, got ",
                          Py_TYPE(x)->tp_name);
-        TORCH_CHECK_VALUE(false, name, "[", i, "] must be a GPU tensor, found ",
-                          THPVariable_Unpack(x).device());
+        TORCH_CHECK_VALUE(THPVariable_Unpack(x).is_cuda(), name, "[", i,
+                          "] must be a GPU tensor, found ", THPVariable_Unpack(x).device());
+        check_plain(THPVariable_Unpack(x), name);
       }
     }
   }
@@ -52,6 +68,7 @@ class List {
 std::optional<at::Tensor> maybe(PyObject* obj, const char* name) {
   if (obj == Py_None) return std::nullopt;
   TORCH_CHECK_TYPE(THPVariable_Check(obj), name, " must be a tensor or None");
+  check_plain(THPVariable_Unpack(obj), name);
   return THPVariable_Unpack(obj);
 }
 
@@ -73,6 +90,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                         &scale, &found))
     return nullptr;
   TORCH_CHECK_TYPE(THPVariable_Check(step), "step must be a tensor");
+  check_plain(THPVariable_Unpack(step), "step");
   o.lr_dev = maybe(lr_dev, "lr");
   o.norm = maybe(norm, "norm");
   o.grad_scale = maybe(scale, "grad_scale");

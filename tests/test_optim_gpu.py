@@ -331,6 +331,21 @@ def test_refusals(cuda):
     assert step.item() == 1.0
 
 
+def test_tensors_whose_memory_is_not_their_values_are_refused(cuda):
+    """Negated views and zeros without memory: the kernels would take what lies there."""
+    x = torch.ones(8, device=cuda)
+    step = torch.zeros((), device=cuda)
+    for odd in (torch._neg_view(x), torch._efficientzerotensor((8,), device=cuda)):
+        with pytest.raises(ValueError, match="holds its values"):
+            optim.grad_norm([x, odd])
+        with pytest.raises(ValueError, match="holds its values"):
+            optim.adamw_step([x.clone()], [odd], [x.clone()], [x.clone()], step, lr=0.1)
+    with pytest.raises(ValueError, match="norm must be a tensor that holds"):
+        optim.adamw_step([x.clone()], [x], [x.clone()], [x.clone()], step, lr=0.1,
+                         norm=torch._neg_view(step), max_norm=1.0)
+    assert step.item() == 0.0
+
+
 # ---- streams, graphs, versions ----------------------------------------------------------------
 
 
