@@ -170,6 +170,12 @@ def head_cross_entropy(hidden, weight, labels, *, ignore_index=-100, reduction="
     return loss.view(labels.shape) if reduction == "none" else loss
 
 
+def _watched(module):
+    """Whether somebody sees the module's calls: hooks, or a forward put on the object itself."""
+    return bool(module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or
+                module._backward_pre_hooks or "forward" in vars(module))
+
+
 def _takes(model, labels, logits_to_keep, kwargs):
     """Whether the patched forward serves this call: a training call for the loss of all positions
     from a plain head in a type the kernels take, with nothing asked for beside it."""
@@ -178,7 +184,10 @@ def _takes(model, labels, logits_to_keep, kwargs):
             and isinstance(logits_to_keep, int) and logits_to_keep == 0):
         return False
     if type(head) is not torch.nn.Linear or head.bias is not None or head.in_features % 64 or \
-            not head.weight.is_cuda or kwargs.get("return_dict") is False:
+            not head.weight.is_cuda or _watched(head):
+        return False
+    asked = kwargs.get("return_dict")  # None: as the configuration says
+    if not (getattr(model.config, "return_dict", True) if asked is None else asked):
         return False
     if kwargs.get("output_hidden_states") or kwargs.get("output_attentions") or \
             getattr(model.config, "output_hidden_states", False) or \
@@ -192,8 +201,10 @@ def _takes(model, labels, logits_to_keep, kwargs):
 def patch_qwen2_head_ce():
     """Qwen2ForCausalLM's training forward takes its loss from head_cross_entropy and returns no
     logits (the reference's patch of the same method); evaluation, generation and calls that ask
-    for more run the original.  Returns whether transformers' Qwen2 model is importable."""
+    for more, models with a loss_function of their own and heads with hooks run the original.
+    Returns whether transformers' Qwen2 model is importable."""
     try:
+        from transformers.loss.loss_utils import ForCausalLMLoss
         from transformers.modeling_outputs import CausalLMOutputWithPast
         from transformers.models.qwen2 import modeling_qwen2
     except Exception:
@@ -206,7 +217,8 @@ def patch_qwen2_head_ce():
     def forward(self, input_ids=None, attention_mask=None, position_ids=None,
                 past_key_values=None, inputs_embeds=None, labels=None, use_cache=None,
                 logits_to_keep=0, **kwargs):
-        if not _takes(self, labels, logits_to_keep, kwargs):
+        if not _takes(self, labels, logits_to_keep, kwargs) or \
+                self.loss_function is not ForCausalLMLoss:
             return original(self, input_ids, attention_mask, position_ids, past_key_values,
                             inputs_embeds, labels, use_cache, logits_to_keep, **kwargs)
         count = kwargs.pop("num_items_in_batch", None)

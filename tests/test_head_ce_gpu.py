@@ -539,6 +539,23 @@ def test_qwen2_training_loss_without_logits(cuda, patched):
     assert model(input_ids=ids, labels=labels).logits is not None
 
 
+def test_qwen2_calls_that_ask_for_more_run_the_original(cuda, patched):
+    """A loss function of the model's own, a hook on the head, and tuples instead of outputs."""
+    model = _tiny_model(BF16).train()
+    ids = torch.randint(1000, (2, 20), device="cuda")
+    assert model(input_ids=ids, labels=ids).logits is None
+    seen = []
+    hook = model.lm_head.register_forward_hook(lambda *a: seen.append(a[2].shape))
+    assert model(input_ids=ids, labels=ids).logits is not None
+    assert len(seen) == 1 and seen[0][:2] == ids.shape
+    hook.remove()
+    out = model(input_ids=ids, labels=ids, return_dict=False)
+    assert isinstance(out, tuple) and out[1].shape[:2] == ids.shape
+    assert model(input_ids=ids, labels=ids, return_dict=None).logits is None  # as configured
+    model.loss_function = lambda logits, labels, **kw: logits.float().sum() * 0 + 7
+    assert model(input_ids=ids, labels=ids).loss.item() == 7.0
+
+
 def test_training_step_end_to_end(cuda, patched):
     """The step's end as a program runs it, all operators in a row: head and loss, gradients,
     their norm, clipping and AdamW with 8-bit states; every matrix moves and stays finite,
