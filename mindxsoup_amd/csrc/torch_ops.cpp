@@ -34,6 +34,7 @@
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -1934,11 +1935,34 @@ struct FusedHeadCE : public torch::autograd::Function<FusedHeadCE> {
   }
 };
 
+// A leaf's accumulator belongs to the stream of the first graph that is alive and uses it.  Where
+// that is the default stream, the backward of a captured call would wait on it inside the capture,
+// which HIP forbids, and the error surfaces where torch can only end the process.
+void check_capture(const Tensor& t, const char* name) {
+  if (!t.is_cuda() || !t.requires_grad() || t.grad_fn()) return;
+  const auto current = c10::hip::getCurrentHIPStream(t.device().index());
+  if (current.id() == 0) return;  // the default stream is never captured
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(current.stream(), &status) != hipSuccess ||
+      status == hipStreamCaptureStatusNone)
+    return;
+  const auto sum = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!sum) return;
+  const auto stream = sum->stream();
+  TORCH_CHECK(!stream.has_value() || stream->id() != 0, name,
+              " is used by an autograd graph that was made on the default stream and is still "
+              "alive: its gradient cannot be captured; let go of that graph first");
+}
+
 Tensor head_cross_entropy_autograd(const Tensor& hidden, const Tensor& weight,
                                    const Tensor& labels, int64_t ignore_index,
                                    int64_t reduction) {
   head_ce_check(hidden, weight, labels, reduction);
   const bool on = at::GradMode::is_enabled();
+  if (on) {
+    check_capture(hidden, "hidden");
+    check_capture(weight, "weight");
+  }
   return FusedHeadCE::apply(hidden, weight, labels, ignore_index, reduction,
                             on && hidden.requires_grad(), on && weight.requires_grad());
 }

@@ -151,7 +151,11 @@ def head_cross_entropy(hidden, weight, labels, *, ignore_index=-100, reduction="
     reduction: "mean" over the positions that take part (NaN if there is none), "sum", or "none":
     fp32 losses in labels' shape, 0 at ignored positions.
     Gradients flow to hidden and, where it requires one, to weight, each summed in fp32 and
-    rounded once."""
+    rounded once.
+
+    The call and its backward can be captured into a graph, as long as no autograd graph that was
+    made from the same leaves on the default stream is still alive (the compiled operator refuses
+    the call then)."""
     if reduction not in REDUCTIONS:
         raise ValueError(f"reduction is one of {REDUCTIONS}, got {reduction!r}")
     for name, t in (("hidden", hidden), ("weight", weight), ("labels", labels)):

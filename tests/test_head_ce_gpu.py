@@ -463,6 +463,27 @@ def test_captured_forward_and_backward(cuda, trained):
         assert all(map(torch.equal, kept, eager)), seed
 
 
+@pytest.mark.parametrize("leaf", ["hidden", "weight"])
+def test_capture_beside_a_living_graph_is_refused(cuda, leaf):
+    """On the default stream: the captured backward would end the process.  Nothing is captured."""
+    h, w, y = _case(60, 300, 64, F16)
+    (h if leaf == "hidden" else w).requires_grad_(True)
+    alive = fused_ce.head_cross_entropy(h, w, y)
+    with pytest.raises(RuntimeError, match=leaf + " is used by an autograd graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            fused_ce.head_cross_entropy(h, w, y)
+    value = alive.item()
+    alive.backward()  # the living one goes on
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fused_ce.head_cross_entropy(h, w, y)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert out.item() == value
+
+
 def test_two_streams_at_once(cuda):
     cases = [_case(300, 2000, 128, F16, seed=i) for i in range(4)]
     want = [_check(*c) for c in cases]
