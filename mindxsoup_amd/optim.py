@@ -97,6 +97,12 @@ def zero_state8(param):
                      for _ in range(2))
 
 
+def _not_captured(p, what):
+    """Tensors that a capture makes are made anew by every replay: states would start over."""
+    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"AdamW: {what} cannot be captured; take it before the capture")
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update (decoupled weight decay, no amsgrad) on `adamw_step`.
 
@@ -104,7 +110,8 @@ class AdamW(torch.optim.Optimizer):
     8 bits.  max_grad_norm clips the gradients of all groups by their global norm within the
     step, without a pass of its own over them.  lr may be a one-value fp32 tensor on the device.
     Parameters whose gradient is None are passed over, and their step count with them.
-    GradScaler hands its scale and its overflow flag to the step instead of unscaling."""
+    GradScaler hands its scale and its overflow flag to the step instead of unscaling.
+    A step can be captured into a graph once each of its parameters has taken one."""
 
     _step_supports_amp_scaling = True
 
@@ -143,6 +150,7 @@ class AdamW(torch.optim.Optimizer):
                 if p.grad.is_sparse:
                     raise RuntimeError("AdamW takes no sparse gradients")
                 if not st:
+                    _not_captured(p, "a parameter's first step")
                     st.update(self._new_state(p, group))
                     if p.device not in fresh:
                         fresh[p.device] = torch.zeros((), dtype=torch.float32, device=p.device)
@@ -156,6 +164,8 @@ class AdamW(torch.optim.Optimizer):
                 continue
             step = self.state[live[0]]["step"]
             if len(live) < len(ps):
+                _not_captured(live[0],
+                              "a step of some of the parameters that stepped together so far")
                 step = step.clone()
             kinds = {}
             for p in live:

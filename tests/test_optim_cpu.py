@@ -30,6 +30,15 @@ def test_optimizer_refuses_bad_arguments(kw):
         optim.AdamW([torch.nn.Parameter(torch.zeros(2))], **kw)
 
 
+@pytest.mark.parametrize("kw", [{}, dict(state_bits=8), dict(max_grad_norm=1.0)])
+def test_optimizer_refuses_cpu_parameters(kw):
+    p = torch.nn.Parameter(torch.ones(5000))
+    p.grad = torch.ones(5000)
+    with pytest.raises(ValueError, match="GPU"):
+        optim.AdamW([p], **kw).step()
+    assert bool((p == 1).all())
+
+
 def test_meta_shapes():
     mx = ops.load()
     g = torch.empty(5, 7, device="meta", dtype=torch.bfloat16)

@@ -380,6 +380,43 @@ def test_captured_step_replays_like_eager(cuda, bits):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer_captured_after_a_first_step(cuda, bits):
+    """Replays go on where eager steps would; what a replay would start anew is refused."""
+    def make():
+        ps = [torch.nn.Parameter(torch.linspace(-1, 1, n, device=cuda)) for n in (5000, 300)]
+        for i, p in enumerate(ps):
+            p.grad = torch.full_like(p, 0.25 + i)
+        return ps, optim.AdamW(ps, lr=1e-2, state_bits=bits, max_grad_norm=1.0)
+
+    ps, opt = make()
+    with pytest.raises(RuntimeError, match="first step cannot be captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    assert not any(opt.state[p] for p in ps)
+    want, eager = make()
+    opt.step()
+    eager.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for k in range(1, 4):
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert all(map(torch.equal, ps, want))
+        assert opt.state[ps[0]]["step"].item() == 1 + k
+    some, opt = make()
+    opt.param_groups[0]["state_bits"] = 32  # both share a step count
+    opt.step()
+    some[1].grad = None
+    with pytest.raises(RuntimeError, match="stepped together"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    opt.step()
+    assert [opt.state[p]["step"].item() for p in some] == [2.0, 1.0]
+
+
 def test_side_stream(cuda):
     p, g, m, v = _case(torch.float32, [50000])
     q, n, w = p[0].clone(), m[0].clone(), v[0].clone()
